@@ -102,6 +102,23 @@ SIGNATURES = {
     "hmoe_combine_workspace_bytes": (c_size_t, [ShapeP]),
     "hmoe_combine": (c_int, [ShapeP, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                              c_size_t, c_void_p]),
+    "hmoe_mxfp4_row_bytes": (c_int32, [c_int32]),
+    "hmoe_mxfp4_quantize": (c_int, [c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p,
+                                    c_void_p]),
+    "hmoe_mxfp4_dequantize": (c_int, [c_void_p, c_int64, c_int32, c_int32, c_void_p, c_void_p]),
+    "hmoe_mxfp4_weight_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32]),
+    "hmoe_mxfp4_pack_weight": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int32,
+                                       c_int32, c_int32, c_void_p, c_void_p]),
+    "hmoe_grouped_linear_mxfp4": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32,
+                                          c_int32, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "hmoe_grouped_swiglu_mxfp4": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32,
+                                          c_int32, c_int32, c_void_p, c_void_p, c_size_t,
+                                          c_void_p]),
+    "hmoe_experts_mxfp4_workspace_bytes": (c_size_t, [ShapeP]),
+    "hmoe_experts_forward_mxfp4": (c_int, [ShapeP] + [c_void_p] * 10 + [c_size_t, c_void_p]),
+    "hmoe_ffn_mxfp4_workspace_bytes": (c_size_t, [ShapeP]),
+    "hmoe_ffn_forward_mxfp4": (c_int, [ShapeP] + [c_void_p] * 6 + [c_int] + [c_void_p] * 5
+                               + [c_size_t, c_void_p]),
     "hmoe_workspace_status": (c_int, [c_void_p, c_void_p]),
     "hmoe_set_pdl_mask": (ctypes.c_uint, [ctypes.c_uint]),
     "hmoe_ep_symmetric_bytes": (c_size_t, [ShapeP, c_int64, c_int32]),

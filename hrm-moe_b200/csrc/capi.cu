@@ -18,6 +18,7 @@
 #include "common.cuh"
 #include "hrm_moe.h"
 #include "internal.h"
+#include "mxfp4.cuh"
 
 using namespace hmoe;
 
@@ -1326,6 +1327,277 @@ int hmoe_workspace_status(const void* workspace, void* stream) {
 unsigned hmoe_set_pdl_mask(unsigned mask) {
   return hmoe::pdl_mask().exchange(mask & (hmoe::kPdlRouter | hmoe::kPdlDispatch | hmoe::kPdlGemm |
                                            hmoe::kPdlCombine));
+}
+
+// ------------------------------------------------------------------- MXFP4 ----
+namespace {
+
+// Restores the calling thread's device: the MXFP4 entry points run on the
+// device of their tensors and leave the current device as it was.
+struct DeviceScope {
+  int prev = -1;
+  DeviceScope() {
+    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+  }
+  ~DeviceScope() {
+    int cur = -1;
+    if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
+  }
+};
+
+int mx_check_k(int64_t K) {
+  if (K <= 0 || K % 8 != 0 || K > (1 << 24))
+    return fail(HMOE_EINVAL, "K must be a positive multiple of 8 (at most 2^24), got %lld",
+                (long long)K);
+  return HMOE_OK;
+}
+
+int mx_check_weight(int32_t groups, int32_t N, int32_t K, int swiglu) {
+  int rc = mx_check_k(K);
+  if (rc) return rc;
+  if (groups <= 0 || groups > 1024) return fail(HMOE_EINVAL, "groups must be in [1, 1024], got %d", groups);
+  if (N <= 0 || N % 8 != 0 || N > (1 << 24))
+    return fail(HMOE_EINVAL, "N must be a positive multiple of 8 (at most 2^24), got %d", N);
+  if (static_cast<int64_t>(groups) * mx_weight_rows(N, swiglu) > 0x7fffffffll)
+    return fail(HMOE_EINVAL, "groups * weight rows must fit in int32");
+  return HMOE_OK;
+}
+
+int mx_grouped(const void* rows, const void* weight, const int32_t* tpe, int64_t M, int32_t N,
+               int32_t K, int32_t G, int swiglu, int quantized_out, void* output, void* workspace,
+               size_t workspace_bytes, void* stream) {
+  int rc = mx_check_weight(G, N, K, swiglu);
+  if (rc) return rc;
+  if (M < 0 || M > 0x7fffffffll) return fail(HMOE_EINVAL, "M must be in [0, 2^31), got %lld", (long long)M);
+  if ((cdiv64(M, 128) + G) * cdiv64(mx_weight_rows(N, swiglu), 64) > 0x7fffffffll)
+    return fail(HMOE_EINVAL, "too many output tiles");
+  if (M == 0) return HMOE_OK;
+  if (!rows || !weight || !tpe || !output) return fail(HMOE_EINVAL, "NULL tensor argument");
+  if (!aligned16(rows) || !aligned16(weight) || !aligned16(output))
+    return fail(HMOE_EINVAL, "rows, weight and output must be 16-byte aligned");
+  DeviceScope scope;
+  if ((rc = select_device(rows))) return rc;
+  int* err = nullptr;
+  if (workspace && workspace_bytes >= sizeof(int)) {
+    err = static_cast<int*>(workspace);
+    HMOE_CUDA(cudaMemsetAsync(err, 0, sizeof(int), static_cast<cudaStream_t>(stream)),
+              "reset error word");
+  }
+  MxGemmArgs a{rows, weight, tpe, output, M, N, K, G, swiglu, quantized_out, err};
+  const cudaError_t e = launch_grouped_gemm_mxfp4(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, swiglu ? "grouped_swiglu_mxfp4" : "grouped_linear_mxfp4");
+  return HMOE_OK;
+}
+
+int mx_validate_shape(const hmoe_shape* s) {
+  int rc = validate_shape(s);
+  if (rc) return rc;
+  if (s->dtype != HMOE_DTYPE_BF16)
+    return fail(HMOE_EINVAL, "the MXFP4 expert path takes bf16 hidden states (dtype %d)", s->dtype);
+  if ((rc = mx_check_weight(s->experts, s->intermediate, s->hidden, 1))) return rc;
+  return mx_check_weight(s->experts, s->hidden, s->intermediate, 0);
+}
+
+struct MxExpertBufs {
+  DispatchBufs d;
+  int32_t* pos;
+  void* xq;   // [T] records of d
+  void* xs;   // [A] records of d, by expert
+  void* h;    // [A] records of I
+  void* out;  // [A, d] bf16: the experts' outputs
+};
+
+MxExpertBufs carve_mx_experts(Carve& c, const hmoe_shape& s) {
+  MxExpertBufs b;
+  const int64_t A = s.tokens * s.top_k;
+  b.d = carve_dispatch(c, s);
+  b.pos = c.take<int32_t>(sizeof(int32_t) * A);
+  b.xq = c.take<void>(static_cast<size_t>(mx_row_bytes(s.hidden)) * s.tokens);
+  b.xs = c.take<void>(static_cast<size_t>(mx_row_bytes(s.hidden)) * A);
+  b.h = c.take<void>(static_cast<size_t>(mx_row_bytes(s.intermediate)) * A);
+  b.out = c.take<void>(2 * static_cast<size_t>(s.hidden) * A);
+  return b;
+}
+
+struct MxFfnBufs {
+  MxExpertBufs x;
+  int32_t* topk_idx;
+  float* topk_w;
+  void* router_scratch;
+};
+
+MxFfnBufs carve_mx_ffn(Carve& c, const hmoe_shape& s) {
+  MxFfnBufs b;
+  const int64_t A = s.tokens * s.top_k;
+  b.x = carve_mx_experts(c, s);
+  b.topk_idx = c.take<int32_t>(sizeof(int32_t) * A);
+  b.topk_w = c.take<float>(sizeof(float) * A);
+  b.router_scratch = c.take<void>(router_tc_scratch_bytes(s.tokens));
+  return b;
+}
+
+// Quantise, dispatch the records, the two products, combine.
+int run_mx_experts(const hmoe_shape& s, const void* x, const int32_t* idx, const void* w,
+                   int w_is_f32, const void* w_gate_up, const void* w_down, const void* final_in,
+                   void* out, int32_t* counts_out, int32_t* sort_idx, const MxExpertBufs& b,
+                   cudaStream_t st) {
+  const int64_t A = s.tokens * s.top_k;
+  HMOE_CUDA(launch_mx_quantize(x, s.tokens, s.hidden, s.hidden, s.dtype, b.xq, st), "quantize_mxfp4");
+  hmoe_shape rec = s;  // dispatch copies records: rows of 2-byte elements
+  rec.hidden = mx_row_bytes(s.hidden) / 2;
+  int rc = run_dispatch(rec, idx, w, w_is_f32, b.xq, b.d, b.pos, sort_idx, nullptr, nullptr, b.xs, st);
+  if (rc) return rc;
+  if (counts_out)
+    HMOE_CUDA(cudaMemcpyAsync(counts_out, b.d.counts, sizeof(int32_t) * s.experts,
+                              cudaMemcpyDeviceToDevice, st), "copy counts");
+  MxGemmArgs gu{b.xs, w_gate_up, b.d.counts, b.h, A, s.intermediate, s.hidden, s.experts, 1, 1, b.d.err};
+  HMOE_CUDA(launch_grouped_gemm_mxfp4(gu, st), "grouped_swiglu_mxfp4");
+  MxGemmArgs dn{b.h, w_down, b.d.counts, b.out, A, s.hidden, s.intermediate, s.experts, 0, 0, b.d.err};
+  HMOE_CUDA(launch_grouped_gemm_mxfp4(dn, st), "grouped_linear_mxfp4");
+  HMOE_CUDA(launch_combine_f32(b.out, b.pos, w, w_is_f32, s.tokens, s.hidden, s.top_k, final_in, out,
+                               st), "combine");
+  return HMOE_OK;
+}
+
+}  // namespace
+
+int32_t hmoe_mxfp4_row_bytes(int32_t K) { return mx_check_k(K) ? 0 : mx_row_bytes(K); }
+
+int hmoe_mxfp4_quantize(const void* x, int64_t rows, int32_t K, int64_t x_stride, int32_t dtype,
+                        void* out, void* stream) {
+  int rc = mx_check_k(K);
+  if (rc) return rc;
+  if (rows < 0) return fail(HMOE_EINVAL, "rows must be >= 0, got %lld", (long long)rows);
+  if (dtype != HMOE_DTYPE_BF16 && dtype != HMOE_DTYPE_F32)
+    return fail(HMOE_EINVAL, "unsupported dtype %d (bf16 = 0, f32 = 1)", dtype);
+  if (rows == 0) return HMOE_OK;
+  if (!x || !out) return fail(HMOE_EINVAL, "x and out are required");
+  if (!aligned16(x) || !aligned16(out) || (x_stride * static_cast<int64_t>(elem_size(dtype))) % 16 != 0)
+    return fail(HMOE_EINVAL, "x, its rows and out must be 16-byte aligned");
+  DeviceScope scope;
+  if ((rc = select_device(x))) return rc;
+  HMOE_CUDA(launch_mx_quantize(x, rows, K, x_stride, dtype, out, static_cast<cudaStream_t>(stream)),
+            "quantize_mxfp4");
+  return HMOE_OK;
+}
+
+int hmoe_mxfp4_dequantize(const void* rows_in, int64_t rows, int32_t K, int32_t dtype, void* out,
+                          void* stream) {
+  int rc = mx_check_k(K);
+  if (rc) return rc;
+  if (rows < 0) return fail(HMOE_EINVAL, "rows must be >= 0, got %lld", (long long)rows);
+  if (dtype != HMOE_DTYPE_BF16 && dtype != HMOE_DTYPE_F32)
+    return fail(HMOE_EINVAL, "unsupported dtype %d (bf16 = 0, f32 = 1)", dtype);
+  if (rows == 0) return HMOE_OK;
+  if (!rows_in || !out) return fail(HMOE_EINVAL, "rows and out are required");
+  if (!aligned16(rows_in) || !aligned16(out)) return fail(HMOE_EINVAL, "rows and out must be 16-byte aligned");
+  DeviceScope scope;
+  if ((rc = select_device(rows_in))) return rc;
+  HMOE_CUDA(launch_mx_dequantize(rows_in, rows, K, dtype, out, static_cast<cudaStream_t>(stream)),
+            "dequantize_mxfp4");
+  return HMOE_OK;
+}
+
+size_t hmoe_mxfp4_weight_bytes(int32_t groups, int32_t N, int32_t K, int32_t swiglu) {
+  if (mx_check_weight(groups, N, K, swiglu != 0)) return 0;
+  return static_cast<size_t>(mx_weight_bytes(groups, N, K, swiglu != 0));
+}
+
+int hmoe_mxfp4_pack_weight(const void* codes, int64_t code_stride, const void* scales,
+                           int64_t scale_stride, int32_t groups, int32_t N, int32_t K,
+                           int32_t swiglu, void* out, void* stream) {
+  int rc = mx_check_weight(groups, N, K, swiglu != 0);
+  if (rc) return rc;
+  if (!codes || !scales || !out) return fail(HMOE_EINVAL, "codes, scales and out are required");
+  if (code_stride < mx_code_bytes(K) || scale_stride < mx_num_scales(K))
+    return fail(HMOE_EINVAL, "row strides (%lld, %lld bytes) are shorter than a row of K=%d",
+                (long long)code_stride, (long long)scale_stride, K);
+  if (!aligned16(codes) || code_stride % 16 != 0 || !aligned16(out))
+    return fail(HMOE_EINVAL, "code rows and out must be 16-byte aligned");
+  DeviceScope scope;
+  if ((rc = select_device(codes))) return rc;
+  HMOE_CUDA(launch_mx_pack_weight(codes, code_stride, scales, scale_stride, groups, N, K, swiglu != 0,
+                                  out, static_cast<cudaStream_t>(stream)),
+            "pack_mxfp4_weight");
+  return HMOE_OK;
+}
+
+int hmoe_grouped_linear_mxfp4(const void* rows, const void* weight, const int32_t* tokens_per_expert,
+                              int64_t M, int32_t N, int32_t K, int32_t groups, void* output,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  return mx_grouped(rows, weight, tokens_per_expert, M, N, K, groups, 0, 0, output, workspace,
+                    workspace_bytes, stream);
+}
+
+int hmoe_grouped_swiglu_mxfp4(const void* rows, const void* w_gate_up,
+                              const int32_t* tokens_per_expert, int64_t M, int32_t I, int32_t K,
+                              int32_t groups, int32_t quantized_out, void* output, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  return mx_grouped(rows, w_gate_up, tokens_per_expert, M, I, K, groups, 1, quantized_out ? 1 : 0,
+                    output, workspace, workspace_bytes, stream);
+}
+
+size_t hmoe_experts_mxfp4_workspace_bytes(const hmoe_shape* shape) {
+  if (mx_validate_shape(shape)) return 0;
+  return plan_bytes(shape, [](Carve& c, const hmoe_shape& s) { carve_mx_experts(c, s); });
+}
+
+int hmoe_experts_forward_mxfp4(const hmoe_shape* shape, const void* hidden,
+                               const int32_t* topk_idx, const void* topk_weight,
+                               const void* w_gate_up, const void* w_down, const void* final_in,
+                               void* y, int32_t* counts, int32_t* sort_idx, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  int rc = mx_validate_shape(shape);
+  if (rc) return rc;
+  const hmoe_shape& s = *shape;
+  DeviceScope scope;
+  if (s.tokens == 0) return zero_counts_if_empty(counts, s.experts, stream);
+  if (!hidden || !topk_idx || !topk_weight || !w_gate_up || !w_down || !y)
+    return fail(HMOE_EINVAL, "hidden, topk_idx, topk_weight, the weights and y are required");
+  if (!aligned16(hidden) || !aligned16(w_gate_up) || !aligned16(w_down) || !aligned16(y) ||
+      !aligned16(final_in))
+    return fail(HMOE_EINVAL, "hidden, weights, final_in and y must be 16-byte aligned");
+  if ((rc = select_device(hidden))) return rc;
+  if ((rc = check_ws(workspace, workspace_bytes, hmoe_experts_mxfp4_workspace_bytes(shape)))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  Carve c{static_cast<char*>(workspace)};
+  MxExpertBufs b = carve_mx_experts(c, s);
+  HMOE_CUDA(cudaMemsetAsync(b.d.err, 0, sizeof(int), st), "reset error word");
+  return run_mx_experts(s, hidden, topk_idx, topk_weight, 0, w_gate_up, w_down, final_in, y, counts,
+                        sort_idx, b, st);
+}
+
+size_t hmoe_ffn_mxfp4_workspace_bytes(const hmoe_shape* shape) {
+  if (mx_validate_shape(shape)) return 0;
+  return plan_bytes(shape, [](Carve& c, const hmoe_shape& s) { carve_mx_ffn(c, s); });
+}
+
+int hmoe_ffn_forward_mxfp4(const hmoe_shape* shape, const void* x, const void* w_router,
+                           const void* router_bias, const void* w_gate_up, const void* w_down,
+                           void* y, int accumulate, int32_t* topk_idx, void* topk_weight,
+                           int32_t* counts, int32_t* sort_idx, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  int rc = mx_validate_shape(shape);
+  if (rc) return rc;
+  const hmoe_shape& s = *shape;
+  DeviceScope scope;
+  if (s.tokens == 0) return zero_counts_if_empty(counts, s.experts, stream);
+  if (!x || !w_router || !w_gate_up || !w_down || !y)
+    return fail(HMOE_EINVAL, "x, w_router, w_gate_up, w_down and y are required");
+  if (!aligned16(x) || !aligned16(w_gate_up) || !aligned16(w_down) || !aligned16(y) ||
+      !aligned16(w_router))
+    return fail(HMOE_EINVAL, "x, weights and y must be 16-byte aligned");
+  if ((rc = select_device(x))) return rc;
+  if ((rc = check_ws(workspace, workspace_bytes, hmoe_ffn_mxfp4_workspace_bytes(shape)))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  Carve c{static_cast<char*>(workspace)};
+  MxFfnBufs b = carve_mx_ffn(c, s);
+  int32_t* idx = topk_idx ? topk_idx : b.topk_idx;
+  HMOE_CUDA(run_router(s, x, w_router, router_bias, idx, b.topk_w, topk_weight, nullptr,
+                       b.router_scratch, b.x.d.err, st, true),
+            "router_topk");
+  return run_mx_experts(s, x, idx, b.topk_w, 1, w_gate_up, w_down, accumulate ? y : nullptr, y,
+                        counts, sort_idx, b.x, st);
 }
 
 }  // extern "C"

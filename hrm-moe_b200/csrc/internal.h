@@ -237,6 +237,36 @@ cudaError_t launch_aux_stats(const void* logits, const int32_t* topk_idx, int64_
 cudaError_t launch_colsum_bf16(const void* m, int64_t T, int E, float* partial, int nblocks,
                                void* out, cudaStream_t stream);
 
+// mxfp4.cu, gemm_mxfp4.cu (layouts: mxfp4.cuh) -----------------------------
+// x [rows, K] (row stride x_stride elements) -> row records.
+cudaError_t launch_mx_quantize(const void* x, int64_t rows, int K, int64_t x_stride, int dtype,
+                               void* out, cudaStream_t st);
+// Row records -> values [rows, K].
+cudaError_t launch_mx_dequantize(const void* rows_in, int64_t rows, int K, int dtype, void* out,
+                                 cudaStream_t st);
+// codes / scales of [G, N (2N for swiglu), K] rows -> packed weight.
+cudaError_t launch_mx_pack_weight(const void* codes, int64_t code_stride, const void* scales,
+                                  int64_t scale_stride, int G, int N, int K, int swiglu, void* out,
+                                  cudaStream_t st);
+// out[t] = [final_in[t] +] sum_j w[t, j] * rows[pos[t, j]]; bf16, fp32 sums.
+cudaError_t launch_combine_f32(const void* rows, const int32_t* pos, const void* topk_w,
+                               int topk_w_is_f32, int64_t T, int d, int k, const void* final_in,
+                               void* out, cudaStream_t st);
+struct MxGemmArgs {
+  const void* rows;       // records [M] of K
+  const void* weight;     // packed, G groups of N (2N for swiglu) rows of K
+  const int32_t* counts;  // [G] rows per group, device
+  void* out;              // bf16 [M, N], or records of N (quantized_out)
+  int64_t M;
+  int N;
+  int K;
+  int G;
+  int swiglu;
+  int quantized_out;      // swiglu only
+  int* err;
+};
+cudaError_t launch_grouped_gemm_mxfp4(const MxGemmArgs& args, cudaStream_t st);
+
 // ep_p2p.cu -------------------------------------------------------------
 size_t ep_symmetric_bytes(const ::hmoe_shape& s, int64_t max_tokens, int world);
 size_t ep_workspace_bytes(const ::hmoe_shape& s, int64_t max_tokens, int world);

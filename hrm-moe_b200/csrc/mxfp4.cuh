@@ -1,0 +1,88 @@
+// MXFP4 (OCP Microscaling Formats v1.0): e2m1 elements, one e8m0 scale per
+// block of 32 along K.
+//
+// Activation rows are records: the codes (K' / 2 bytes, low nibble first,
+// K' = K filled up to whole blocks), then one scale byte per block, the scale
+// section filled up to 8 bytes and the record to 16 with zeros.  A record
+// moves as one row copy (dispatch), its codes are 16-byte aligned for TMA, and
+// the 8 scale bytes of a 256-element k-block are one aligned load.
+//
+// Packed weights: the codes [G, N', K' / 2] (for gate_up weights N' =
+// 2 * ceil(I / 32) * 32 with 32 gate rows, then the 32 up rows of the same
+// features, and so on, so that a column tile holds matching gate and up
+// columns), then, 1024-byte aligned, the scales as the tensor core's
+// scale-factor atoms: [G][ceil(N' / 128)][ceil(K' / 256)][2][512], byte
+// (n % 32) * 16 + (n % 128) / 32 * 4 + s of an atom being the scale of row n,
+// block s of the atom's 128 elements.
+#pragma once
+
+#include "common.cuh"
+
+namespace hmoe {
+
+constexpr int kMxBlock = 32;   // elements per scale
+constexpr int kMxKBlock = 256;  // elements per 128-byte swizzled row of codes
+
+__host__ __device__ inline int mx_padded_k(int K) { return (K + 31) / 32 * 32; }
+__host__ __device__ inline int mx_code_bytes(int K) { return mx_padded_k(K) / 2; }
+__host__ __device__ inline int mx_num_scales(int K) { return mx_padded_k(K) / 32; }
+__host__ __device__ inline int mx_scale_bytes(int K) { return (mx_num_scales(K) + 7) / 8 * 8; }
+__host__ __device__ inline int mx_row_bytes(int K) {
+  return (mx_code_bytes(K) + mx_scale_bytes(K) + 15) / 16 * 16;
+}
+// Rows of one group's packed weight for N output columns.
+__host__ __device__ inline int mx_weight_rows(int N, int swiglu) {
+  return swiglu ? 2 * mx_padded_k(N) : N;
+}
+inline int64_t mx_weight_scale_offset(int G, int N, int K, int swiglu) {
+  const int64_t codes = static_cast<int64_t>(G) * mx_weight_rows(N, swiglu) * mx_code_bytes(K);
+  return (codes + 1023) / 1024 * 1024;
+}
+inline int64_t mx_weight_bytes(int G, int N, int K, int swiglu) {
+  return mx_weight_scale_offset(G, N, K, swiglu) +
+         static_cast<int64_t>(G) * cdiv(mx_weight_rows(N, swiglu), 128) *
+             cdiv(mx_padded_k(K), kMxKBlock) * 1024;
+}
+
+// Scale byte of a block whose largest magnitude has the fp32 bits `amax`
+// (sign cleared): floor(log2 amax) - 2, the exponent of e2m1's largest power
+// of two being 2, at least 2^-127; 255 (NaN) when the block holds an infinity
+// or a NaN.  The maximum is taken on the bits: they order as the values do,
+// and NaN comes out above everything.
+__device__ __forceinline__ uint32_t mx_scale_code(uint32_t amax) {
+  const uint32_t e = amax >> 23;
+  return e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+}
+// 1 / scale (exact: a power of two between 2^-125 and 2^127; 0 for NaN).
+__device__ __forceinline__ float mx_inv_scale(uint32_t code) {
+  return code == 255u ? 0.0f : __uint_as_float((254u - code) << 23);
+}
+
+// Eight values -> eight e2m1 codes in one word (v0 in the low nibble), round to
+// nearest even, saturating at 6.
+__device__ __forceinline__ uint32_t mx_cvt8(float v0, float v1, float v2, float v3, float v4,
+                                            float v5, float v6, float v7) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r)
+      : "f"(v0), "f"(v1), "f"(v2), "f"(v3), "f"(v4), "f"(v5), "f"(v6), "f"(v7));
+  return r;
+}
+
+// The value of a 4-bit code, times 2^(scale - 127) (exact).
+__device__ __forceinline__ float mx_value(uint32_t code, uint32_t scale) {
+  const uint32_t m = code & 7u;
+  // e2m1 magnitude: 0, 0.5, 1, 1.5, 2, 3, 4, 6
+  const float mag = m < 2u ? 0.5f * m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
+  if (scale == 255u) return __uint_as_float(0x7fc00000u);
+  // 2^(scale - 127) in two factors: 2^-127 is a subnormal
+  const float s = scale >= 1u ? __uint_as_float(scale << 23) : __uint_as_float(0x00400000u);
+  return (code & 8u ? -mag : mag) * s;
+}
+
+}  // namespace hmoe

@@ -414,6 +414,314 @@ def ffn_forward(x: torch.Tensor, w_router: torch.Tensor, w_gate_up: torch.Tensor
     return (out, routing) if return_routing else out
 
 
+# ------------------------------------------------------------------- MXFP4 --
+def _inference_only(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward (MXFP4 is for inference): call it under "
+                           "torch.no_grad() or torch.inference_mode()")
+
+
+class Mxfp4Rows:
+    """Rows in MXFP4 (OCP MX: e2m1 elements, one e8m0 scale per 32 along the last axis).
+
+    ``data`` [..., row_bytes] uint8 holds one record per row (include/hrm_moe.h);
+    ``codes`` [..., K'/2] (even element in the low nibble) and ``scales``
+    [..., K'/32] (the value is 2^(byte - 127), 255 = NaN) are views of it, K'
+    being K filled up to whole blocks with zeros.
+    """
+
+    def __init__(self, data: torch.Tensor, k: int):
+        row_bytes = _lib.load().hmoe_mxfp4_row_bytes(int(k))
+        if row_bytes == 0:
+            raise ValueError(_lib.last_error())
+        if data.dtype != torch.uint8:
+            raise TypeError(f"MXFP4 records are uint8, got {data.dtype}")
+        if data.dim() < 1 or data.shape[-1] != row_bytes or not data.is_contiguous():
+            raise ValueError(f"MXFP4 records of K={k} are contiguous rows of {row_bytes} bytes, got "
+                             f"{tuple(data.shape)}")
+        self.data = data
+        self.k = int(k)
+
+    @property
+    def shape(self) -> torch.Size:
+        return torch.Size((*self.data.shape[:-1], self.k))
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self.data[..., : -(-self.k // 32) * 16]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        blocks = -(-self.k // 32)
+        return self.data[..., 16 * blocks: 17 * blocks]
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The values the rows stand for (bf16 and fp32 both hold them exactly)."""
+        code = dtype_code(dtype)
+        dev = _require_cuda(self.data)
+        out = torch.empty(self.shape, dtype=dtype, device=dev)
+        _lib.check(_lib.load().hmoe_mxfp4_dequantize(
+            _ptr(self.data), out.numel() // self.k, self.k, code, _ptr(out), _stream(dev)))
+        return out
+
+
+def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Rows:
+    """Rows x [..., K] (bf16 or fp32, K a multiple of 8) to MXFP4 along the last axis.
+
+    A block's scale is 2^(floor(log2 max|x|) - 2); elements round to nearest
+    even and saturate at 6 scales; a block with an infinity or a NaN becomes
+    NaN.
+    """
+    _inference_only("quantize_mxfp4", x)
+    code = dtype_code(x.dtype)
+    dev = _require_cuda(x)
+    if x.dim() < 1:
+        raise ValueError("quantize_mxfp4 takes rows [..., K]")
+    k = x.shape[-1]
+    lib = _lib.load()
+    row_bytes = lib.hmoe_mxfp4_row_bytes(k)
+    if row_bytes == 0:
+        raise ValueError(_lib.last_error())
+    es = x.element_size()
+    if not (x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= k
+            and x.stride(0) * es % 16 == 0 and x.data_ptr() % 16 == 0):
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    data = torch.empty((*x.shape[:-1], row_bytes), dtype=torch.uint8, device=dev)
+    rows = data.numel() // row_bytes
+    _lib.check(lib.hmoe_mxfp4_quantize(_ptr(x), rows, k, x.stride(0) if x.dim() == 2 else k, code,
+                                       _ptr(data), _stream(dev)))
+    return Mxfp4Rows(data, k)
+
+
+class Mxfp4Weight:
+    """An expert weight packed for the MXFP4 products (see :func:`pack_mxfp4_weight`).
+
+    [groups, n, k] for ``grouped_linear_mxfp4``; with ``swiglu`` the gate and
+    up halves of [groups, 2n, k] for ``grouped_swiglu_mxfp4``.
+    """
+
+    def __init__(self, data: torch.Tensor, groups: int, n: int, k: int, swiglu: bool):
+        self.data, self.groups, self.n, self.k, self.swiglu = data, groups, n, k, swiglu
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.data.numel()
+
+
+def pack_mxfp4_weight(weight, k: Optional[int] = None, swiglu: bool = False) -> Mxfp4Weight:
+    """Lay out expert weights [G, N, K] for the MXFP4 products, once, when they are loaded.
+
+    ``weight`` is a bf16 or fp32 tensor (quantised here), :class:`Mxfp4Rows` of
+    shape [G, N, K], or (codes [G, N, K'/2], scales [G, N, K'/32]) uint8 as a
+    checkpoint holds them, with ``k`` = K.  ``swiglu``: the rows are the I gate
+    rows, then the I up rows of each expert (N = 2I), as in
+    ``experts.gate_up_weight``.  The weight is copied: later changes to the
+    source do not reach it.
+    """
+    if isinstance(weight, torch.Tensor):
+        weight = quantize_mxfp4(weight.detach())
+    if isinstance(weight, Mxfp4Rows):
+        k, codes, scales = weight.k, weight.codes, weight.scales
+    else:
+        codes, scales = weight
+        if k is None:
+            raise ValueError("k is required with codes and scales")
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError(f"codes and scales are uint8, got {codes.dtype} and {scales.dtype}")
+        codes, scales = codes.contiguous(), scales.contiguous()
+        if codes.data_ptr() % 16:
+            codes = codes.clone()
+    dev = _require_cuda(codes, scales)
+    blocks = -(-int(k) // 32)
+    if codes.dim() != 3 or codes.shape[2] != 16 * blocks or \
+            tuple(scales.shape) != (*codes.shape[:2], blocks):
+        raise ValueError(f"MXFP4 weight of K={k}: codes {tuple(codes.shape)}, scales "
+                         f"{tuple(scales.shape)}")
+    G, N = codes.shape[:2]
+    if swiglu and N % 2:
+        raise ValueError("gate_up weight needs an even number of rows")
+    n = N // 2 if swiglu else N
+    lib = _lib.load()
+    nbytes = lib.hmoe_mxfp4_weight_bytes(G, n, int(k), int(swiglu))
+    if nbytes == 0:
+        raise ValueError(_lib.last_error())
+    data = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _lib.check(lib.hmoe_mxfp4_pack_weight(_ptr(codes), codes.stride(1), _ptr(scales),
+                                          scales.stride(1), G, n, int(k), int(swiglu), _ptr(data),
+                                          _stream(dev)))
+    return Mxfp4Weight(data, G, n, int(k), bool(swiglu))
+
+
+def _grouped_mxfp4(what: str, x, weight: Mxfp4Weight, tokens_per_expert: torch.Tensor, swiglu: bool,
+                   quantized: bool):
+    if not isinstance(weight, Mxfp4Weight):
+        raise TypeError(f"{what} takes a weight from pack_mxfp4_weight, got {type(weight).__name__}")
+    if weight.swiglu != swiglu:
+        raise ValueError(f"{what} needs a weight packed with swiglu={swiglu}")
+    if not isinstance(x, Mxfp4Rows):
+        _inference_only(what, x)
+        if x.dim() == 2 and x.shape[1] != weight.k:
+            raise ValueError(f"grouped GEMM K mismatch: input K={x.shape[1]}, weight K={weight.k}")
+        x = quantize_mxfp4(x)
+    if len(x.shape) != 2 or x.k != weight.k:
+        raise ValueError(f"grouped GEMM K mismatch: input {tuple(x.shape)}, weight K={weight.k}")
+    if tokens_per_expert.numel() != weight.groups:
+        raise ValueError(f"tokens_per_expert has {tokens_per_expert.numel()} entries, weight has "
+                         f"{weight.groups} groups")
+    dev = _require_cuda(x.data, weight.data, tokens_per_expert)
+    M = x.shape[0]
+    tpe = tokens_per_expert
+    if tpe.dtype != torch.int32 or not tpe.is_contiguous():
+        tpe = tpe.to(torch.int32).contiguous()
+    lib = _lib.load()
+    if quantized:
+        out = torch.empty((M, lib.hmoe_mxfp4_row_bytes(weight.n)), dtype=torch.uint8, device=dev)
+    else:
+        out = torch.empty((M, weight.n), dtype=torch.bfloat16, device=dev)
+    if swiglu:
+        _lib.check(lib.hmoe_grouped_swiglu_mxfp4(
+            _ptr(x.data), _ptr(weight.data), _ptr(tpe), M, weight.n, weight.k, weight.groups,
+            int(quantized), _ptr(out), None, 0, _stream(dev)))
+    else:
+        _lib.check(lib.hmoe_grouped_linear_mxfp4(
+            _ptr(x.data), _ptr(weight.data), _ptr(tpe), M, weight.n, weight.k, weight.groups,
+            _ptr(out), None, 0, _stream(dev)))
+    return Mxfp4Rows(out, weight.n) if quantized else out
+
+
+def grouped_linear_mxfp4(x, weight: Mxfp4Weight, tokens_per_expert: torch.Tensor) -> torch.Tensor:
+    """``grouped_linear`` on MXFP4 operands: [M, K] -> bf16 [M, N], sums in fp32.
+
+    ``x`` is :class:`Mxfp4Rows` or a bf16 / fp32 tensor, which is quantised
+    first; ``tokens_per_expert`` [G] counts each group's rows, contiguous in
+    order.  Inference only.
+    """
+    return _grouped_mxfp4("grouped_linear_mxfp4", x, weight, tokens_per_expert, False, False)
+
+
+def grouped_swiglu_mxfp4(x, weight: Mxfp4Weight, tokens_per_expert: torch.Tensor,
+                         quantized: bool = False):
+    """``grouped_swiglu`` on MXFP4 operands: silu(gate) * up in fp32, [M, K] -> [M, I].
+
+    Returns bf16, or with ``quantized`` the :class:`Mxfp4Rows` the down product
+    takes (quantised from the fp32 values).  Inference only.
+    """
+    return _grouped_mxfp4("grouped_swiglu_mxfp4", x, weight, tokens_per_expert, True, quantized)
+
+
+def _mxfp4_shape(T: int, d: int, dtype: torch.dtype, top_k: int, w_gate_up, w_down,
+                 norm_topk_prob: bool = True) -> _lib.HmoeShape:
+    for w in (w_gate_up, w_down):
+        if not isinstance(w, Mxfp4Weight):
+            raise TypeError(f"expert weights come from pack_mxfp4_weight, got {type(w).__name__}")
+    if dtype != torch.bfloat16:
+        raise TypeError(f"the MXFP4 expert path takes bf16 hidden states, got {dtype}")
+    E, I = w_gate_up.groups, w_gate_up.n
+    if not w_gate_up.swiglu or w_down.swiglu or w_gate_up.k != d or \
+            (w_down.groups, w_down.n, w_down.k) != (E, d, I):
+        raise ValueError(
+            f"expert weights [{E}, {'2 x ' if w_gate_up.swiglu else ''}{I}, {w_gate_up.k}] / "
+            f"[{w_down.groups}, {w_down.n}, {w_down.k}] do not match hidden size {d}")
+    return make_shape(T, d, E, I, top_k, dtype, norm_topk_prob)
+
+
+def experts_forward_mxfp4(hidden_states: torch.Tensor, selected_experts: torch.Tensor,
+                          routing_weights: torch.Tensor, w_gate_up: Mxfp4Weight,
+                          w_down: Mxfp4Weight,
+                          final_hidden_states: Optional[torch.Tensor] = None,
+                          counts_out: Optional[torch.Tensor] = None,
+                          sort_idx_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``experts_forward`` with MXFP4 expert weights; activations are quantised in the call.
+
+    Returns a new [T, d] bf16 tensor, or adds into ``final_hidden_states`` in
+    place and returns it.  The products sum in fp32, each expert's output is
+    bf16, and a token's weighted sum is fp32 rounded once.  Inference only.
+    """
+    _inference_only("experts_forward_mxfp4", hidden_states, routing_weights, final_hidden_states)
+    T, d = hidden_states.shape
+    k = selected_experts.shape[-1]
+    shape = _mxfp4_shape(T, d, hidden_states.dtype, k, w_gate_up, w_down)
+    dev = _require_cuda(hidden_states, selected_experts, routing_weights, final_hidden_states,
+                        w_gate_up.data, w_down.data)
+    out = final_hidden_states
+    if out is None:
+        out = torch.empty((T, d), dtype=torch.bfloat16, device=dev)
+    elif tuple(out.shape) != (T, d) or out.dtype != torch.bfloat16 or not out.is_contiguous():
+        raise ValueError(f"final_hidden_states must be contiguous bf16 [{T}, {d}] (it is updated in "
+                         "place)")
+    if T == 0:
+        return out
+    hs = hidden_states.contiguous()
+    idx = selected_experts.reshape(T, k).to(torch.int32).contiguous()
+    rw = routing_weights.reshape(T, k).to(torch.bfloat16).contiguous()
+    lib = _lib.load()
+    ws_bytes = lib.hmoe_experts_mxfp4_workspace_bytes(ctypes.byref(shape))
+    if ws_bytes == 0:
+        raise ValueError(_lib.last_error())
+    ws = _workspace(ws_bytes, dev)
+    _lib.check(lib.hmoe_experts_forward_mxfp4(
+        ctypes.byref(shape), _ptr(hs), _ptr(idx), _ptr(rw), _ptr(w_gate_up.data),
+        _ptr(w_down.data), _ptr(final_hidden_states), _ptr(out), _ptr(counts_out),
+        _ptr(sort_idx_out), _ptr(ws), ws.numel(), _stream(dev)))
+    return out
+
+
+def ffn_forward_mxfp4(x: torch.Tensor, w_router: torch.Tensor, w_gate_up: Mxfp4Weight,
+                      w_down: Mxfp4Weight, top_k: int, norm_topk_prob: bool,
+                      router_bias: Optional[torch.Tensor] = None,
+                      out: Optional[torch.Tensor] = None, accumulate: bool = False,
+                      return_routing: bool = False):
+    """``ffn_forward`` with MXFP4 expert weights: the bf16 router (same routing), then
+    the experts as in :func:`experts_forward_mxfp4`.  Inference only."""
+    _inference_only("ffn_forward_mxfp4", x, w_router, router_bias)
+    T, d = x.shape
+    dt = x.dtype
+    shape = _mxfp4_shape(T, d, dt, top_k, w_gate_up, w_down, norm_topk_prob)
+    E = w_gate_up.groups
+    if tuple(w_router.shape) != (E, d):
+        raise ValueError(f"router weight is {tuple(w_router.shape)}, expected {(E, d)}")
+    if out is None:
+        out = (torch.zeros if accumulate else torch.empty)((T, d), dtype=dt, device=x.device)
+    elif tuple(out.shape) != (T, d) or out.dtype != dt or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {dt} [{T}, {d}]")
+    routing = None
+    if T == 0:
+        return (out, routing) if return_routing else out
+    dev = _require_cuda(x, w_router, w_gate_up.data, w_down.data, router_bias, out)
+    x = x.contiguous()
+    w_router = w_router.to(dt).contiguous()
+    bias = None if router_bias is None else router_bias.to(dt).contiguous()
+    if return_routing:
+        routing = {
+            "topk_idx": torch.empty((T, top_k), dtype=torch.int32, device=dev),
+            "topk_weight": torch.empty((T, top_k), dtype=dt, device=dev),
+            "counts": torch.empty(E, dtype=torch.int32, device=dev),
+            "sort_idx": torch.empty(T * top_k, dtype=torch.int32, device=dev),
+        }
+    r = routing or {}
+    lib = _lib.load()
+    ws_bytes = lib.hmoe_ffn_mxfp4_workspace_bytes(ctypes.byref(shape))
+    if ws_bytes == 0:
+        raise ValueError(_lib.last_error())
+    ws = _workspace(ws_bytes, dev)
+    _lib.check(lib.hmoe_ffn_forward_mxfp4(
+        ctypes.byref(shape), _ptr(x), _ptr(w_router), _ptr(bias), _ptr(w_gate_up.data),
+        _ptr(w_down.data), _ptr(out), 1 if accumulate else 0, _ptr(r.get("topk_idx")),
+        _ptr(r.get("topk_weight")), _ptr(r.get("counts")), _ptr(r.get("sort_idx")), _ptr(ws),
+        ws.numel(), _stream(dev)))
+    return (out, routing) if return_routing else out
+
+
 # ---------------------------------------------------------------- training --
 def _train_shape(x, w_router, w_gate_up, w_down, top_k, norm_topk_prob):
     T, d = x.shape
@@ -552,7 +860,8 @@ class CapturedFfn:
     the graph's input and ``y`` its output; ``__call__(x)`` copies ``x`` into
     the input (same shape and dtype), replays the graph on the current stream
     and returns ``y`` (overwritten by the next call).  Same kernels and
-    results as :func:`ffn_forward`.
+    results as :func:`ffn_forward`, or, with weights from
+    :func:`pack_mxfp4_weight`, as :func:`ffn_forward_mxfp4`.
     """
 
     def __init__(self, x: torch.Tensor, w_router: torch.Tensor, w_gate_up: torch.Tensor,
@@ -561,21 +870,32 @@ class CapturedFfn:
         T, d = x.shape
         if T == 0:
             raise ValueError("nothing to capture for 0 tokens")
-        dev = _require_cuda(x, w_router, w_gate_up, w_down, router_bias)
         dt = x.dtype
         E = w_router.shape[0]
-        I = w_gate_up.shape[1] // 2
-        if tuple(w_gate_up.shape) != (E, 2 * I, d) or tuple(w_down.shape) != (E, d, I):
-            raise ValueError(f"expert weights {tuple(w_gate_up.shape)} / {tuple(w_down.shape)} do "
-                             f"not match hidden size {d} and {E} experts")
+        self._mxfp4 = isinstance(w_gate_up, Mxfp4Weight) or isinstance(w_down, Mxfp4Weight)
+        if self._mxfp4:
+            self._shape = _mxfp4_shape(T, d, dt, top_k, w_gate_up, w_down, norm_topk_prob)
+            if tuple(w_router.shape) != (w_gate_up.groups, d):
+                raise ValueError(f"router weight is {tuple(w_router.shape)}, expected "
+                                 f"{(w_gate_up.groups, d)}")
+            w_gate_up, w_down = w_gate_up.data, w_down.data
+            dev = _require_cuda(x, w_router, w_gate_up, w_down, router_bias)
+        else:
+            dev = _require_cuda(x, w_router, w_gate_up, w_down, router_bias)
+            I = w_gate_up.shape[1] // 2
+            if tuple(w_gate_up.shape) != (E, 2 * I, d) or tuple(w_down.shape) != (E, d, I):
+                raise ValueError(f"expert weights {tuple(w_gate_up.shape)} / {tuple(w_down.shape)} "
+                                 f"do not match hidden size {d} and {E} experts")
+            self._shape = _lib.HmoeShape(T, d, E, I, top_k, dtype_code(dt),
+                                         1 if norm_topk_prob else 0)
+            w_gate_up, w_down = w_gate_up.to(dt).contiguous(), w_down.to(dt).contiguous()
         self.x_static = x.detach().clone().contiguous()
         self.y = torch.empty_like(self.x_static)
-        self._w = [w_router.to(dt).contiguous(), w_gate_up.to(dt).contiguous(),
-                   w_down.to(dt).contiguous(),
+        self._w = [w_router.to(dt).contiguous(), w_gate_up, w_down,
                    None if router_bias is None else router_bias.to(dt).contiguous()]
-        self._shape = _lib.HmoeShape(T, d, E, I, top_k, dtype_code(dt), 1 if norm_topk_prob else 0)
         lib = _lib.load()
-        nbytes = lib.hmoe_ffn_workspace_bytes(ctypes.byref(self._shape))
+        nbytes = (lib.hmoe_ffn_mxfp4_workspace_bytes if self._mxfp4
+                  else lib.hmoe_ffn_workspace_bytes)(ctypes.byref(self._shape))
         if nbytes == 0:
             raise ValueError(_lib.last_error())
         self._ws = _workspace(nbytes, dev)
@@ -591,7 +911,8 @@ class CapturedFfn:
     def _launch(self, stream: torch.cuda.Stream) -> None:
         wr, wgu, wd, b = self._w
         lib = _lib.load()
-        _lib.check(lib.hmoe_ffn_forward(
+        fn = lib.hmoe_ffn_forward_mxfp4 if self._mxfp4 else lib.hmoe_ffn_forward
+        _lib.check(fn(
             ctypes.byref(self._shape), _ptr(self.x_static), _ptr(wr), _ptr(b), _ptr(wgu), _ptr(wd),
             _ptr(self.y), 0, None, None, None, None, _ptr(self._ws), self._ws.numel(),
             ctypes.c_void_p(stream.cuda_stream)))

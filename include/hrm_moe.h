@@ -382,6 +382,77 @@ int hmoe_ffn_backward_marked(const hmoe_shape* shape, const void* grad_y, const 
                              void* stream, void* const* phase_events);
 
 /*
+ * MXFP4 expert products (inference).  No counterpart in the reference, whose
+ * expert weights are bf16 or fp32.  Format: OCP Microscaling Formats v1.0,
+ * e2m1 elements with one e8m0 scale (2^(byte - 127), 255 = NaN) per block of
+ * 32 along K; the scale of a block is 2^(floor(log2 max|x|) - 2), at least
+ * 2^-127; elements round to nearest even and saturate at 6; a block with an
+ * infinity or a NaN gets the NaN scale; a last block shorter than 32 is filled
+ * up with zeros (K' = K rounded up to 32).  K is a multiple of 8.
+ *
+ * Row records (hmoe_mxfp4_row_bytes(K) bytes each, contiguous, 16-byte
+ * aligned): K'/2 bytes of codes (the even element in the low nibble), K'/32
+ * scale bytes, zeros up to the record's size.  hmoe_mxfp4_quantize makes them
+ * from x [rows, K] (bf16 or fp32, x_stride elements from row to row, rows
+ * 16-byte aligned); hmoe_mxfp4_dequantize gives their values back (bf16 holds
+ * them exactly).
+ *
+ * Packed weights (opaque, hmoe_mxfp4_weight_bytes, 16-byte aligned) are laid
+ * out once by hmoe_mxfp4_pack_weight from codes and scales in row order: rows
+ * [G, N, K] (swiglu = 0) or [G, 2N, K], gate rows then up rows (swiglu = 1),
+ * code_stride / scale_stride bytes from row to row.  A checkpoint's MXFP4
+ * tensors and the two parts of row records both have that form.
+ */
+int32_t hmoe_mxfp4_row_bytes(int32_t K);
+int hmoe_mxfp4_quantize(const void* x, int64_t rows, int32_t K, int64_t x_stride, int32_t dtype,
+                        void* out, void* stream);
+int hmoe_mxfp4_dequantize(const void* rows_in, int64_t rows, int32_t K, int32_t dtype, void* out,
+                          void* stream);
+size_t hmoe_mxfp4_weight_bytes(int32_t groups, int32_t N, int32_t K, int32_t swiglu);
+int hmoe_mxfp4_pack_weight(const void* codes, int64_t code_stride, const void* scales,
+                           int64_t scale_stride, int32_t groups, int32_t N, int32_t K,
+                           int32_t swiglu, void* out, void* stream);
+
+/*
+ * hmoe_grouped_linear / hmoe_grouped_swiglu on MXFP4 operands: rows [M] are
+ * records of K, weight a packed weight (swiglu = 0 / 1).  Sums in fp32.
+ *   linear: output [M, N] bf16
+ *   swiglu: h = silu(gate) * up in fp32; output [M, I] bf16, or with
+ *           quantized_out [M] records of I (the next product's rows)
+ * Rows past the last group are left as they were; groups past row M are cut
+ * off.  N and K multiples of 8.  Workspace as hmoe_grouped_linear.
+ */
+int hmoe_grouped_linear_mxfp4(const void* rows, const void* weight,
+                              const int32_t* tokens_per_expert, int64_t M, int32_t N, int32_t K,
+                              int32_t groups, void* output, void* workspace,
+                              size_t workspace_bytes, void* stream);
+int hmoe_grouped_swiglu_mxfp4(const void* rows, const void* w_gate_up,
+                              const int32_t* tokens_per_expert, int64_t M, int32_t I, int32_t K,
+                              int32_t groups, int32_t quantized_out, void* output,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * hmoe_experts_forward / hmoe_ffn_forward with packed MXFP4 expert weights
+ * (w_gate_up: swiglu = 1, I = intermediate, K = hidden; w_down: swiglu = 0,
+ * N = hidden, K = intermediate).  bf16 hidden states, quantised within the
+ * call; the routing is that of hmoe_ffn_forward.
+ *   y[t] = bf16([final_in[t] +] sum_j w[t, j] * bf16(down(MXFP4(h))))
+ * summed in fp32 and rounded once.  final_in may be NULL (nothing added) or y.
+ */
+size_t hmoe_experts_mxfp4_workspace_bytes(const hmoe_shape* shape);
+int hmoe_experts_forward_mxfp4(const hmoe_shape* shape, const void* hidden,
+                               const int32_t* topk_idx, const void* topk_weight,
+                               const void* w_gate_up, const void* w_down, const void* final_in,
+                               void* y, int32_t* counts, int32_t* sort_idx, void* workspace,
+                               size_t workspace_bytes, void* stream);
+size_t hmoe_ffn_mxfp4_workspace_bytes(const hmoe_shape* shape);
+int hmoe_ffn_forward_mxfp4(const hmoe_shape* shape, const void* x, const void* w_router,
+                           const void* router_bias, const void* w_gate_up, const void* w_down,
+                           void* y, int accumulate, int32_t* topk_idx, void* topk_weight,
+                           int32_t* counts, int32_t* sort_idx, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/*
  * Read (and synchronise the stream for) the error word kernels leave at the
  * start of a workspace used by hmoe_ffn_forward, hmoe_experts_forward,
  * hmoe_dispatch, hmoe_grouped_* or hmoe_ep_forward: HMOE_OK, HMOE_EINVAL (an
