@@ -244,12 +244,7 @@ int run_dispatch(const hmoe_shape& s, const int32_t* idx, const void* w, int w_i
 // pair from T=2048).  HMOE_GEMM_KERNEL=pair or =single (read once per
 // process) forces one kernel.
 bool use_cta_pair_gemm(int64_t M, int G) {
-  static const int forced = [] {
-    const char* v = std::getenv("HMOE_GEMM_KERNEL");
-    if (v && std::strcmp(v, "pair") == 0) return 1;
-    if (v && std::strcmp(v, "single") == 0) return 0;
-    return -1;
-  }();
+  const int forced = forced_gemm_kernel();
   if (forced >= 0) return forced == 1;
   return M > 192 * static_cast<int64_t>(G);
 }
@@ -351,6 +346,16 @@ std::atomic<unsigned>& pdl_mask() {
              : static_cast<unsigned>(kPdlRouter | kPdlDispatch | kPdlGemm);
   }()};
   return mask;
+}
+
+int forced_gemm_kernel() {
+  static const int forced = [] {
+    const char* v = std::getenv("HMOE_GEMM_KERNEL");
+    if (v && std::strcmp(v, "pair") == 0) return 1;
+    if (v && std::strcmp(v, "single") == 0) return 0;
+    return -1;
+  }();
+  return forced;
 }
 
 bool pdl_enabled(unsigned cls) { return (pdl_mask().load(std::memory_order_relaxed) & cls) != 0; }

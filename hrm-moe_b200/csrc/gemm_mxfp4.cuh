@@ -1,0 +1,330 @@
+// Shared pieces of the MXFP4 grouped GEMMs: block-scaled MMA wrappers, tile
+// tables, the epilogue of 32 output columns, tensor maps.
+#pragma once
+
+#include <cuda.h>
+#include <mutex>
+
+#include "internal.h"
+#include "mxfp4.cuh"
+
+namespace hmoe {
+namespace mx {
+
+constexpr int MM = 128;      // rows of one CTA's tile
+constexpr int kRowB = 128;   // bytes of codes per operand row and k-block
+constexpr int kMaxGroups = 1024;
+constexpr int kAtom = 512;   // scales of 128 rows x 128 elements
+constexpr int kEpiBox = 32 * 32 * 2;
+constexpr int kTmemCols = 512;
+
+struct Params {
+  const uint8_t* a_rows;    // records
+  const uint8_t* b_scales;  // atoms
+  const int32_t* counts;
+  int G;
+  int64_t M;
+  int N;            // output columns
+  int K;
+  int a_row_bytes;
+  int a_box_rows;   // rows of one A load (single-CTA kernel)
+  int n_tiles;
+  int tile_chunks;  // 64-column chunks of a column tile (pair kernel); the first
+  int tile_extra;   // tile_extra tiles have one more
+  int b_rows;       // packed rows per group
+  int b_chunks;     // 128-row scale chunks per group
+  void* out;        // bf16 [M, N] or records
+  int* err;
+  unsigned long long wait_limit_ns;
+};
+
+__device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                         uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], "
+      "p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_mxf4_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                              uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], "
+      "p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// 32 rows x 16 bytes of shared memory to four TMEM columns of all four lane
+// quadrants (the pair form: in both CTAs, each from its own shared memory).
+__device__ __forceinline__ void tmem_cp_atom(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_cp_atom_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+               : "memory");
+}
+// One lane of a converged warp, chosen by the hardware.  Around the issue of
+// TMA and tcgen05 instructions this, not a test of the lane index: the
+// compiler then knows that a single lane is active and emits each instruction
+// once, instead of a loop over the active lanes (measured in the pair kernel:
+// 110 -> 50 cycles per tcgen05 instruction issued).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
+// Scale atom in shared memory: no swizzle, 8-row core matrices of 128
+// contiguous bytes.
+__device__ __forceinline__ uint64_t smem_desc_atom(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(128u >> 4) << 16;
+  d |= static_cast<uint64_t>(128u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  return d;
+}
+// Instruction descriptor of the block-scaled kinds: bits [4,6) B scale id,
+// [7,10) A type (1 = e2m1), [10,12) B type, [17,23) N >> 3, 23 scale type
+// (1 = e8m0), [27,29) M >> 7, [29,31) A scale id.
+__host__ __device__ constexpr uint32_t idesc_mxf4(int m, int n, int sf_id) {
+  return (static_cast<uint32_t>(sf_id) << 4) | (1u << 7) | (1u << 10) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) |
+         (static_cast<uint32_t>(m >> 7) << 27) | (static_cast<uint32_t>(sf_id) << 29);
+}
+__device__ __forceinline__ void st_shared_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void st_shared_v4m(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z),
+               "r"(v.w)
+               : "memory");
+}
+
+struct GroupTables {
+  int group_rows[kMaxGroups + 1];
+  int tile_prefix[kMaxGroups + 1];  // prefix of row blocks
+  int num_m_tiles;
+};
+
+// One warp: the groups' first rows and row blocks from the device counts.
+// Rows past M are cut off, so that no count, however wrong, leads outside the
+// operands.
+__device__ __forceinline__ void build_tables(GroupTables& t, const int32_t* counts, int G, int64_t M,
+                                             int block_rows) {
+  const int lane = threadIdx.x & 31;
+  const int per = cdiv(G, 32);
+  const int g0 = min(G, lane * per), g1 = min(G, g0 + per);
+  int64_t rows = 0;
+  for (int g = g0; g < g1; ++g) rows += max(0, counts[g]);
+  int64_t rin = rows;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t ro = __shfl_up_sync(0xffffffffu, rin, off);
+    if (lane >= off) rin += ro;
+  }
+  int64_t rr = rin - rows;
+  int tiles = 0;
+  for (int g = g0; g < g1; ++g) {
+    const int a = static_cast<int>(rr < M ? rr : M);
+    rr += max(0, counts[g]);
+    const int b = static_cast<int>(rr < M ? rr : M);
+    t.group_rows[g] = a;
+    t.tile_prefix[g] = tiles;
+    tiles += cdiv(b - a, block_rows);
+  }
+  int tin = tiles;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int to = __shfl_up_sync(0xffffffffu, tin, off);
+    if (lane >= off) tin += to;
+  }
+  for (int g = g0; g < g1; ++g) t.tile_prefix[g] += tin - tiles;
+  if (lane == 31) {
+    t.group_rows[G] = static_cast<int>(rin < M ? rin : M);
+    t.tile_prefix[G] = tin;
+    t.num_m_tiles = tin;
+  }
+}
+
+struct RowBlock {
+  int g, row0, row_end;
+};
+__device__ __forceinline__ RowBlock find_block(const GroupTables& t, int G, int mt, int block_rows) {
+  int lo = 0, hi = G;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.tile_prefix[mid] <= mt) lo = mid; else hi = mid;
+  }
+  RowBlock r;
+  r.g = lo;
+  r.row0 = t.group_rows[lo] + (mt - t.tile_prefix[lo]) * block_rows;
+  r.row_end = t.group_rows[lo + 1];
+  return r;
+}
+
+// silu(g) * u = g * u / (1 + 2^(-g log2 e)), in fp32 with the hardware's
+// approximate exponential and reciprocal (2^-22 relative each; the
+// denominator is at least 1, so flushing subnormals changes nothing).
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return g * r * u;
+}
+
+// max(|a|, |b|, c), NaN if any is.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 32 output columns of one row, as a warp: quantised to a record's block, or
+// rounded to bf16 and stored as a whole 32 x 32 box by TMA where all 32 rows
+// are the group's, else row by row.
+template <bool QOUT>
+__device__ __forceinline__ void store_chunk(const float (&v)[32], const Params& p,
+                                            const CUtensorMap* tmC, int col0, int64_t row,
+                                            int box_row, bool row_ok, bool box_full, uint32_t stg) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (QOUT) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max3_abs(v[2 * i], v[2 * i + 1], m);
+    const uint32_t s = mx_scale_code(__float_as_uint(m));
+    const float inv = mx_inv_scale(s);
+    uint32_t q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      q[i] = mx_cvt8(v[8 * i] * inv, v[8 * i + 1] * inv, v[8 * i + 2] * inv, v[8 * i + 3] * inv,
+                     v[8 * i + 4] * inv, v[8 * i + 5] * inv, v[8 * i + 6] * inv,
+                     v[8 * i + 7] * inv);
+    if (row_ok) {
+      const int row_bytes = mx_row_bytes(p.N), cb = mx_code_bytes(p.N), ns = mx_num_scales(p.N);
+      uint8_t* orow = static_cast<uint8_t*>(p.out) + row * row_bytes;
+      *reinterpret_cast<uint4*>(orow + col0 / 2) = make_uint4(q[0], q[1], q[2], q[3]);
+      orow[cb + col0 / 32] = static_cast<uint8_t>(s);
+      if (col0 / 32 == ns - 1)
+        for (int b = cb + ns; b < row_bytes; ++b) orow[b] = 0;
+    }
+  } else {
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = cvt_bf16x2(v[2 * i], v[2 * i + 1]);
+    if (box_full) {
+      if (lane == 0) bulk_wait_group_read<0>();
+      __syncwarp();
+      const uint32_t dst = stg + lane * 64;
+      const uint32_t sw = (lane >> 1) & 3;
+#pragma unroll
+      for (int c4 = 0; c4 < 4; ++c4)
+        st_shared_v4m(dst + ((c4 ^ sw) << 4),
+                      make_uint4(w[4 * c4], w[4 * c4 + 1], w[4 * c4 + 2], w[4 * c4 + 3]));
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d(tmC, col0, box_row, stg);
+        bulk_commit_group();
+      }
+    } else if (row_ok) {
+      uint16_t* orow = static_cast<uint16_t*>(p.out) + row * p.N;
+#pragma unroll
+      for (int c4 = 0; c4 < 4; ++c4)
+        if (col0 + c4 * 8 + 8 <= p.N)
+          *reinterpret_cast<uint4*>(orow + col0 + c4 * 8) =
+              make_uint4(w[4 * c4], w[4 * c4 + 1], w[4 * c4 + 2], w[4 * c4 + 3]);
+    }
+  }
+}
+
+// 32 output columns out of TMEM: 32 accumulator columns, or (SWIGLU) the 32
+// gate columns and the 32 up columns behind them.
+template <bool SWIGLU>
+__device__ __forceinline__ void load_chunk(uint32_t taddr, float (&v)[32]) {
+  uint32_t ra[32];
+  tmem_ld_32cols(taddr, ra);
+  if constexpr (SWIGLU) {
+    uint32_t ua[32];
+    tmem_ld_32cols(taddr + 32, ua);
+    tc_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = silu_mul(__uint_as_float(ra[i]), __uint_as_float(ua[i]));
+  } else {
+    tc_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(ra[i]);
+  }
+}
+
+// ------------------------------------------------------------ host side ----
+bool make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t rows,
+              uint64_t cols, uint64_t stride, uint32_t box_rows, uint32_t box_cols,
+              CUtensorMapSwizzle swizzle);
+// Scale chunks of 1024 bytes [rows][nkb]: boxes of two rows' chunks of one k-block.
+bool make_scale_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t nkb);
+// Codes [rows, cols bytes] with a row stride, boxes of box_rows x 128 bytes.
+inline bool make_code_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
+                          uint64_t stride, uint32_t box_rows) {
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rows, cols, stride, box_rows, kRowB,
+                  CU_TENSOR_MAP_SWIZZLE_128B);
+}
+inline bool make_out_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols) {
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, rows, cols, cols * 2, 32, 32,
+                  CU_TENSOR_MAP_SWIZZLE_64B);
+}
+inline Params make_params(const MxGemmArgs& a) {
+  Params p;
+  p.a_rows = static_cast<const uint8_t*>(a.rows);
+  p.b_scales = static_cast<const uint8_t*>(a.weight) +
+               mx_weight_scale_offset(a.G, a.N, a.K, a.swiglu);
+  p.counts = a.counts;
+  p.G = a.G;
+  p.M = a.M;
+  p.N = a.N;
+  p.K = a.K;
+  p.a_row_bytes = mx_row_bytes(a.K);
+  p.a_box_rows = MM;
+  p.b_rows = mx_weight_rows(a.N, a.swiglu);
+  p.b_chunks = cdiv(p.b_rows, 128);
+  p.n_tiles = p.tile_chunks = p.tile_extra = 0;
+  p.out = a.out;
+  p.err = a.err;
+  p.wait_limit_ns = kWaitLimitNs;
+  return p;
+}
+
+// Once per kernel and device: the shared-memory opt-in.
+template <class Kernel>
+cudaError_t allow_smem(Kernel kernel, size_t bytes, int (&done)[64], std::mutex& mu) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> lock(mu);
+  if (!done[dev]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(bytes));
+    if (e != cudaSuccess) return e;
+    done[dev] = 1;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace mx
+
+// 256-row tiles on CTA pairs (gemm_mxfp4_pair.cu).
+cudaError_t launch_grouped_gemm_mxfp4_pair(const MxGemmArgs& args, cudaStream_t st);
+
+}  // namespace hmoe

@@ -278,6 +278,8 @@ cudaError_t ep_forward_launch(const ::hmoe_shape& s, int64_t max_tokens, int ran
 
 // capi.cu ---------------------------------------------------------------
 int num_sms_for_current_device();
+// HMOE_GEMM_KERNEL (read once per process): 1 pair, 0 single, -1 not set.
+int forced_gemm_kernel();
 // Entry-point plumbing for files other than capi.cu: set hmoe_last_error()
 // and return `code`; make the device owning `ptr` current (sm_100 only);
 // validate a shape.

@@ -135,6 +135,14 @@ CASES = [
     (4099, 200, 1000, 5, 1),
     (4096, 1536, 512, 64, 5),
     (9000, 328, 1536, 128, 30),
+    # groups of many rows: CTA pairs
+    (1000, 8, 8, 1, 0),
+    (1025, 136, 264, 2, 0),
+    (257, 64, 1536, 1, 0),
+    (3000, 72, 2056, 3, 1),
+    (1500, 320, 1800, 2, 0),
+    (5001, 1536, 512, 8, 2),
+    (30000, 512, 1536, 64, 3),
 ]
 
 
@@ -177,6 +185,26 @@ def test_grouped_swiglu(M, N, K, G, zeros):
     room = R.flip_room(h, tol)
     assert (off <= room).all(), (off - room).max()
     assert np.mean(off > 0) < 1e-3 or off.size < 10000
+
+
+def test_cta_pair_and_single_cta_kernels_agree(tmp_path):
+    """The two kernels give the same bits (child processes that force one each:
+    HMOE_GEMM_KERNEL is read once per process)."""
+    import os
+    import subprocess
+    import sys
+
+    import mxfp4_kernels_worker_gpu as W
+
+    outs = {}
+    for kern in ("pair", "single"):
+        path = tmp_path / f"{kern}.pt"
+        env = dict(os.environ, HMOE_GEMM_KERNEL=kern)
+        subprocess.run([sys.executable, W.__file__, str(path)], env=env, check=True, timeout=600)
+        outs[kern] = torch.load(path)
+    assert outs["pair"].keys() == outs["single"].keys()
+    for key in outs["pair"]:
+        assert torch.equal(outs["pair"][key], outs["single"][key]), key
 
 
 def test_checkpoint_and_rows_pack_alike():
