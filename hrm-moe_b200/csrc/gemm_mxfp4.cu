@@ -4,40 +4,37 @@
 //   SwiGLU:  h = silu(x @ gate^T) * (x @ up^T), in fp32           -> bf16 or
 //            MXFP4 records (the next product's input; h never exists in bf16)
 //
-// One persistent CTA per SM, 128-row tiles.  A k-block is 256 elements: a
-// 128-byte swizzled row of codes per operand row.  Warp 0 loads A (row
-// records through a tensor map whose row stride is the record), B and B's
-// scale atoms; warps 2-3 bring A's scales (row-major in the records, 8 bytes
-// per row and k-block) into the atom layout; warp 1 copies the atoms to TMEM
-// and issues the MMAs; eight warps run the epilogue.  Each stage has its own
-// TMEM scale columns, so a stage's empty barrier covers its scales as well.
+// This file: one persistent CTA per SM, tiles of 128 rows x (up to) 192
+// columns, for groups of few rows.  (CTA pairs, for groups of many:
+// gemm_mxfp4_pair.cu.)  A k-block is 256 elements: a 128-byte swizzled row of
+// codes per operand row.  Warp 0 loads A (row records through a tensor map
+// whose row stride is the record; only the 32-row boxes that the group
+// reaches), A's scales as the records hold them, B and B's scale atoms; warp 2
+// brings A's scales into the atom layout; warp 3 copies the atoms to TMEM;
+// warp 1 issues the MMAs; twelve warps run the epilogue.  Each stage has its
+// own TMEM scale columns, so a stage's empty barrier covers its scales as well.
 #include "gemm_mxfp4.cuh"
 
 namespace hmoe {
 namespace mx {
 namespace {
 
-constexpr int kThreads = 384;  // 4 control warps, 8 epilogue warps
-constexpr int kAccs = 2;
+constexpr int ST = 4;          // stages
+constexpr int kRaw = 3;        // pairs of k-blocks of A's scales as they come
+constexpr int kABytes = MM * kRowB;
+constexpr int kBBytes = kAccCols * kRowB;
+constexpr int kOffSfa = kABytes + kBBytes;  // in a stage
+constexpr int kOffSfb = kOffSfa + 2 * kAtom;
+constexpr int kStageBytes = (kOffSfb + kSfbBytes + 1023) / 1024 * 1024;
+constexpr int kSfCol = kAccs * kAccCols;
+constexpr int kSfCols = kSfaCols + kSfbCols;  // of a stage
+static_assert(kSfCol + ST * kSfCols <= kTmemCols, "TMEM columns");
 
-template <int BN>
-struct Tile {
-  static constexpr int kStages = 5;
-  static constexpr int kNB = (BN + 127) / 128;  // scale chunks of B
-  static constexpr int kABytes = MM * kRowB;
-  static constexpr int kBBytes = BN * kRowB;
-  static constexpr int kSfA = 2 * kAtom;
-  static constexpr int kSfB = 2 * kAtom * kNB;
-  static constexpr int kStageBytes = kABytes + kBBytes + kSfA + kSfB;
-  static constexpr int kSfCols = 8 + 8 * kNB;  // TMEM scale columns of a stage
-  static constexpr int kSfBase = kAccs * BN;
-  static_assert(kSfBase + kStages * kSfCols <= kTmemCols, "TMEM columns");
-};
-
-template <int STAGES>
 struct Ctl {
-  uint64_t full[STAGES];
-  uint64_t empty[STAGES];
+  uint64_t full[ST];
+  uint64_t empty[ST];
+  uint64_t sf_full[ST];  // the stage's scales are in TMEM
+  uint64_t raw_full[kRaw], raw_empty[kRaw];
   uint64_t acc_full[kAccs];
   uint64_t acc_empty[kAccs];
   uint64_t drain;
@@ -45,13 +42,11 @@ struct Ctl {
   int abort;
   GroupTables tab;
 };
-
-template <int BN>
-constexpr size_t smem_bytes() {
-  return 1024 + static_cast<size_t>(Tile<BN>::kStages) * Tile<BN>::kStageBytes +
-         8 * kEpiBox + sizeof(Ctl<Tile<BN>::kStages>);
-}
-static_assert(smem_bytes<128>() <= 232448, "shared memory budget of one sm_100 CTA");
+constexpr int kOffRaw = ST * kStageBytes;  // [128 rows][16 scales]
+constexpr int kOffEpi = kOffRaw + kRaw * 2048;
+constexpr int kOffCtl = kOffEpi + kEpiWarps * kEpiBox;
+constexpr size_t kSmemBytes = 1024 + kOffCtl + sizeof(Ctl);
+static_assert(kSmemBytes <= 232448, "shared memory budget of one sm_100 CTA");
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
                                           uint32_t bar) {
@@ -61,54 +56,60 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
       "l"(src), "r"(bytes), "r"(bar)
       : "memory");
 }
-struct TilePos : RowBlock {
-  int n;
+struct Tile : RowBlock {
+  int c0, nc;  // 64-column chunks
 };
-__device__ __forceinline__ TilePos decode_tile(const GroupTables& tab, int G, int n_tiles, int tile) {
-  const int mt = tile / n_tiles;
-  TilePos t;
-  static_cast<RowBlock&>(t) = find_block(tab, G, mt, MM);
-  t.n = tile - mt * n_tiles;
+__device__ __forceinline__ Tile decode_tile(const GroupTables& tab, const Params& p, int tile) {
+  const int mt = tile / p.ct.tiles;
+  const int n = tile - mt * p.ct.tiles;
+  Tile t;
+  static_cast<RowBlock&>(t) = find_block(tab, p.G, mt, MM);
+  t.c0 = p.ct.first(n);
+  t.nc = p.ct.count(n);
   return t;
 }
 
-template <int BN, bool SWIGLU, bool QOUT>
+template <bool SWIGLU, bool QOUT>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
                           const __grid_constant__ CUtensorMap tmB,
+                          const __grid_constant__ CUtensorMap tmR,
                           const __grid_constant__ CUtensorMap tmC, const Params p) {
-  using T = Tile<BN>;
-  constexpr int ST = T::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  auto& ctl = *reinterpret_cast<Ctl<ST>*>(smem + ST * T::kStageBytes + 8 * kEpiBox);
+  Ctl& ctl = *reinterpret_cast<Ctl*>(smem + kOffCtl);
   const uint32_t sbase = smem_u32(smem);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int G = p.G;
 
   // ---------------------------------------------------------------- setup
   if (warp == 0) {
     if (lane == 0) {
       for (int s = 0; s < ST; ++s) {
-        mbar_init(smem_u32(&ctl.full[s]), 3);   // the producer's arm, two scale warps
+        mbar_init(smem_u32(&ctl.full[s]), 2);   // the producer's arm, the scale warp
         mbar_init(smem_u32(&ctl.empty[s]), 1);  // one commit per stage use
+        mbar_init(smem_u32(&ctl.sf_full[s]), 1);
+      }
+      for (int s = 0; s < kRaw; ++s) {
+        mbar_init(smem_u32(&ctl.raw_full[s]), 1);
+        mbar_init(smem_u32(&ctl.raw_empty[s]), 1);
       }
       for (int a = 0; a < kAccs; ++a) {
         mbar_init(smem_u32(&ctl.acc_full[a]), 1);
-        mbar_init(smem_u32(&ctl.acc_empty[a]), 8);  // the epilogue warps
+        mbar_init(smem_u32(&ctl.acc_empty[a]), kEpiWarps);
       }
       mbar_init(smem_u32(&ctl.drain), 1);
       ctl.abort = 0;
       fence_mbar_init();
       tma_prefetch_desc(&tmA);
       tma_prefetch_desc(&tmB);
+      tma_prefetch_desc(&tmR);
       tma_prefetch_desc(&tmC);
     }
     __syncwarp();
     grid_dependency_wait();  // launched early (launch_pdl): the counts are written before this
-    build_tables(ctl.tab, p.counts, G, p.M, MM);
+    build_tables(ctl.tab, p.counts, p.G, p.M, MM);
   } else if (warp == 1) {
     tmem_alloc(smem_u32(&ctl.tmem_base), kTmemCols);
   }
@@ -118,189 +119,184 @@ grouped_gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
   grid_dependency_wait();
   grid_launch_dependents();
 
-  const uint32_t tmem_base = ctl.tmem_base;
-  const int num_tiles = ctl.tab.num_m_tiles * p.n_tiles;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl.tmem_base, 0);
+  const int num_tiles = ctl.tab.num_m_tiles * p.ct.tiles;
   const int kp = mx_padded_k(p.K);
-  const int nkb = cdiv(kp, kMxKBlock);
+  const int nkb = mx_num_kblocks(p.K);
   volatile int* abort = &ctl.abort;
   int never = 0;
   const unsigned long long lim = p.wait_limit_ns;
+  const auto wait = [&](uint64_t& bar, uint32_t parity) {
+    return mbar_wait_bounded(smem_u32(&bar), parity, abort, p.err, lim);
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (elect_one()) {
-      int stage = 0;
-      uint32_t phase = 0;
+      Ring st, raw;
       bool ok = true;
+      const int soff = mx_code_bytes(p.K);
       for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
-        const TilePos t = decode_tile(ctl.tab, G, p.n_tiles, tile);
+        const Tile t = decode_tile(ctl.tab, p, tile);
         const int boxes = cdiv(min(MM, t.row_end - t.row0), p.a_box_rows);
-        const int brow = t.g * p.b_rows + t.n * BN;
-        const int nchunks = min(T::kNB, p.b_chunks - t.n * BN / 128);
-        const uint8_t* bs = p.b_scales +
-                            (static_cast<int64_t>(t.g) * p.b_chunks + t.n * BN / 128) * nkb * 1024;
-        const uint32_t bytes = boxes * p.a_box_rows * kRowB + T::kBBytes + nchunks * 1024;
+        const int brow = t.g * p.b_rows + t.c0 * 64;
+        const uint8_t* bs =
+            p.b_scales + (static_cast<int64_t>(t.g) * p.b_chunks + t.c0) * nkb * kAtom;
+        // B in boxes of 64 rows
+        const uint32_t bytes = boxes * p.a_box_rows * kRowB + t.nc * (64 * kRowB + kAtom);
         for (int kb = 0; kb < nkb; ++kb) {
-          if (!mbar_wait_bounded(smem_u32(&ctl.empty[stage]), phase ^ 1u, abort, p.err, lim)) {
+          if ((kb & 1) == 0) {  // A's scales of two k-blocks
+            if (!wait(ctl.raw_empty[raw.slot], raw.phase ^ 1u)) {
+              ok = false;
+              break;
+            }
+            const uint32_t rb = smem_u32(&ctl.raw_full[raw.slot]);
+            mbar_arrive_expect_tx(rb, boxes * p.a_box_rows * 16);
+            for (int b = 0; b < boxes; ++b)
+              tma_load_2d(sbase + kOffRaw + raw.slot * 2048 + b * p.a_box_rows * 16, &tmR,
+                          soff + kb * 8, t.row0 + b * p.a_box_rows, rb);
+            raw.next(kRaw);
+          }
+          if (!wait(ctl.empty[st.slot], st.phase ^ 1u)) {
             ok = false;
             break;
           }
-          const uint32_t fb = smem_u32(&ctl.full[stage]);
-          const uint32_t sa = sbase + stage * T::kStageBytes;
+          const uint32_t fb = smem_u32(&ctl.full[st.slot]);
+          const uint32_t sa = sbase + st.slot * kStageBytes;
           mbar_arrive_expect_tx(fb, bytes);
+          for (int c = 0; c < t.nc; ++c)
+            tma_load_2d(sa + kABytes + c * 64 * kRowB, &tmB, kb * kRowB, brow + c * 64, fb);
+          bulk_load(sa + kOffSfb, bs + static_cast<int64_t>(kb) * t.nc * kAtom, t.nc * kAtom, fb);
           for (int b = 0; b < boxes; ++b)
-            tma_load_2d(sa + b * p.a_box_rows * kRowB, &tmA, kb * kRowB,
-                        t.row0 + b * p.a_box_rows, fb);
-          tma_load_2d(sa + T::kABytes, &tmB, kb * kRowB, brow, fb);
-          for (int c = 0; c < nchunks; ++c)
-            bulk_load(sa + T::kABytes + T::kBBytes + T::kSfA + c * 1024,
-                      bs + (static_cast<int64_t>(c) * nkb + kb) * 1024, 1024, fb);
-          if (++stage == ST) { stage = 0; phase ^= 1u; }
+            tma_load_2d(sa + b * p.a_box_rows * kRowB, &tmA, kb * kRowB, t.row0 + b * p.a_box_rows, fb);
+          st.next(ST);
         }
       }
-      // wait until every stage filled has been released by the MMAs
-      for (int i = 0; i < ST; ++i) {
-        if (!mbar_wait_bounded(smem_u32(&ctl.empty[stage]), phase ^ 1u, &never, p.err, lim)) break;
-        if (++stage == ST) { stage = 0; phase ^= 1u; }
-      }
+      // wait until every stage filled has been released
+      for (int i = 0; i < ST; ++i, st.next(ST))
+        if (!mbar_wait_bounded(smem_u32(&ctl.empty[st.slot]), st.phase ^ 1u, &never, p.err, lim)) break;
+      for (int i = 0; i < kRaw; ++i, raw.next(kRaw))
+        if (!mbar_wait_bounded(smem_u32(&ctl.raw_empty[raw.slot]), raw.phase ^ 1u, &never, p.err, lim)) break;
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
     if (elect_one()) {
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
+      Ring st, acc;
       bool ok = true;
+      const uint64_t adesc0 = smem_desc_sw128(sbase);
       for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
-        if (!mbar_wait_bounded(smem_u32(&ctl.acc_empty[acc]), acc_phase ^ 1u, abort, p.err, lim))
-          break;
+        const int nc = p.ct.count(tile % p.ct.tiles);
+        const uint32_t id0 = idesc_mxf4(MM, 64 * nc, 0), id1 = idesc_mxf4(MM, 64 * nc, 2);
+        if (!wait(ctl.acc_empty[acc.slot], acc.phase ^ 1u)) break;
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc.slot * kAccCols);
         for (int kb = 0; kb < nkb; ++kb) {
-          if (!mbar_wait_bounded(smem_u32(&ctl.full[stage]), phase, abort, p.err, lim)) {
+          // committed by a thread that has waited for the stage's operands
+          if (!wait(ctl.sf_full[st.slot], st.phase)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sa = sbase + stage * T::kStageBytes;
-          const uint32_t sb = sa + T::kABytes;
-          const uint32_t ssfa = sb + T::kBBytes, ssfb = ssfa + T::kSfA;
-          const uint32_t tsfa = tmem_base + T::kSfBase + stage * T::kSfCols, tsfb = tsfa + 8;
-          // the scales of 128 elements: four columns per 128 rows
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            tmem_cp_atom(tsfa + 4 * j, smem_desc_atom(ssfa + j * kAtom));
-#pragma unroll
-            for (int c = 0; c < T::kNB; ++c)
-              tmem_cp_atom(tsfb + 4 * T::kNB * j + 4 * c,
-                           smem_desc_atom(ssfb + c * 1024 + j * kAtom));
-          }
+          const uint64_t ad = adesc0 + st.slot * (kStageBytes >> 4), bd = ad + (kABytes >> 4);
+          const uint32_t tsfa = tmem_base + kSfCol + st.slot * kSfCols, tsfb = tsfa + kSfaCols;
           const int mmas = min(4, cdiv(kp - kb * kMxKBlock, 64));
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
             if (kk >= mmas) break;
-            mma_mxf4(d_tmem, smem_desc_sw128(sa + kk * 32), smem_desc_sw128(sb + kk * 32),
-                     idesc_mxf4(MM, BN, (kk & 1) * 2), tsfa + 4 * (kk >> 1),
-                     tsfb + 4 * T::kNB * (kk >> 1), (kb | kk) != 0 ? 1u : 0u);
+            mma_mxf4(d_tmem, ad + 2 * kk, bd + 2 * kk, (kk & 1) ? id1 : id0, tsfa + 4 * (kk >> 1),
+                     tsfb + 2 * nc * (kk >> 1), (kb | kk) != 0 ? 1u : 0u);
           }
-          tc_commit(smem_u32(&ctl.empty[stage]));
-          if (++stage == ST) { stage = 0; phase ^= 1u; }
+          tc_commit(smem_u32(&ctl.empty[st.slot]));
+          st.next(ST);
         }
         if (!ok) break;
-        tc_commit(smem_u32(&ctl.acc_full[acc]));
-        if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
+        tc_commit(smem_u32(&ctl.acc_full[acc.slot]));
+        acc.next(kAccs);
       }
       // every MMA issued has completed before TMEM is freed
       tc_commit(smem_u32(&ctl.drain));
       mbar_wait_bounded(smem_u32(&ctl.drain), 0, &never, p.err, lim);
     }
-  } else if (warp < 4) {
-    // ------------------------------------------------------ scales of A
-    // Thread i brings rows i and i + 64: batches of four k-blocks, the next
-    // batch's loads in flight while this one is stored.
-    const int r0 = (warp - 2) * 32 + lane;
-    const int soff = mx_code_bytes(p.K);
-    int stage = 0;
-    uint32_t phase = 0;
-    uint2 cur[2][4], nxt[2][4];
-    auto load = [&](int tile, int kb0, uint2 (&v)[2][4]) {
-      const TilePos t = decode_tile(ctl.tab, G, p.n_tiles, tile);
+  } else if (warp == 3) {
+    // ------------------------------------------- scales from shared memory to TMEM
+    if (elect_one()) {
+      Ring st;
+      bool ok = true;
+      const uint64_t sf0 = smem_desc_atom(sbase + kOffSfa);
+      for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
+        const int nc = p.ct.count(tile % p.ct.tiles);
+        for (int kb = 0; kb < nkb; ++kb) {
+          if (!wait(ctl.full[st.slot], st.phase)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t sfa = sf0 + st.slot * (kStageBytes >> 4), sfb = sfa + (2 * kAtom >> 4);
+          const uint32_t tsfa = tmem_base + kSfCol + st.slot * kSfCols, tsfb = tsfa + kSfaCols;
+          tmem_cp_atom(tsfa, sfa);
+          tmem_cp_atom(tsfa + 4, sfa + (kAtom >> 4));
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = t.row0 + r0 + 64 * h;
-        const uint8_t* src = p.a_rows + static_cast<int64_t>(row) * p.a_row_bytes + soff;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v[h][i] = row < t.row_end && kb0 + i < nkb
-                        ? *reinterpret_cast<const uint2*>(src + (kb0 + i) * 8)
-                        : make_uint2(0, 0);
+          for (int c = 0; c < kMxTileChunks; ++c)
+            if (c < nc) tmem_cp_atom(tsfb + 4 * c, sfb + c * (kAtom >> 4));
+          tc_commit(smem_u32(&ctl.sf_full[st.slot]));
+          st.next(ST);
+        }
       }
-    };
-    int tile = blockIdx.x, kb0 = 0;
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------ scales of A
+    // From the records' order into the atoms': lane i moves rows i, i + 32,
+    // i + 64, i + 96, whose words make up one lane of an atom.
+    Ring st, raw;
     bool ok = true;
-    if (tile < num_tiles) load(tile, 0, cur);
-    while (ok && tile < num_tiles) {
-      int ntile = tile, nkb0 = kb0 + 4;
-      if (nkb0 >= nkb) { nkb0 = 0; ntile += gridDim.x; }
-      if (ntile < num_tiles) load(ntile, nkb0, nxt);
+    for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
+      uint4 v[4];
+      for (int kb = 0; kb < nkb; ++kb) {
+        if ((kb & 1) == 0) {
+          if (!wait(ctl.raw_full[raw.slot], raw.phase)) {
+            ok = false;
+            break;
+          }
+          const uint4* src = reinterpret_cast<const uint4*>(smem + kOffRaw + raw.slot * 2048) + lane;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (kb0 + i >= nkb) break;
-        if (!mbar_wait_bounded(smem_u32(&ctl.empty[stage]), phase ^ 1u, abort, p.err, lim)) {
+          for (int h = 0; h < 4; ++h) v[h] = src[32 * h];
+        }
+        if (!wait(ctl.empty[st.slot], st.phase ^ 1u)) {
           ok = false;
           break;
         }
-        const uint32_t dst = sbase + stage * T::kStageBytes + T::kABytes + T::kBBytes + lane * 16;
+        const uint32_t dst = sbase + st.slot * kStageBytes + kOffSfa + lane * 16;
+        st_shared_v4m(dst, make_uint4(v[0].x, v[1].x, v[2].x, v[3].x));
+        st_shared_v4m(dst + kAtom, make_uint4(v[0].y, v[1].y, v[2].y, v[3].y));
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t d = dst + ((warp - 2) + 2 * h) * 4;
-          st_shared_u32(d, cur[h][i].x);
-          st_shared_u32(d + kAtom, cur[h][i].y);
-        }
+        for (int h = 0; h < 4; ++h) { v[h].x = v[h].z; v[h].y = v[h].w; }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&ctl.full[stage]));
-        if (++stage == ST) { stage = 0; phase ^= 1u; }
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&ctl.full[st.slot]));
+          // only here: the stores have taken the values, so the loads are done
+          // (an arrival right behind the loads let the next copy overtake them)
+          if ((kb & 1) == 0) mbar_arrive(smem_u32(&ctl.raw_empty[raw.slot]));
+        }
+        if ((kb & 1) == 0) raw.next(kRaw);
+        st.next(ST);
       }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) cur[h][i] = nxt[h][i];
-      tile = ntile;
-      kb0 = nkb0;
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    const int quad = warp & 3;
-    const int half = (warp - 4) >> 2;
-    const int r_in_tile = quad * 32 + lane;
-    const uint32_t stg = sbase + ST * T::kStageBytes + (warp - 4) * kEpiBox;
-    int acc = 0;
-    uint32_t acc_phase = 0;
+    const int w = warp - 4;
+    const uint32_t stg = sbase + kOffEpi + w * kEpiBox;
+    Ring acc;
     for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x) {
-      const TilePos t = decode_tile(ctl.tab, G, p.n_tiles, tile);
-      const int nrows = min(MM, t.row_end - t.row0);
-      if (!mbar_wait_bounded(smem_u32(&ctl.acc_full[acc]), acc_phase, abort, p.err, lim)) break;
+      const Tile t = decode_tile(ctl.tab, p, tile);
+      if (!wait(ctl.acc_full[acc.slot], acc.phase)) break;
       tc_fence_after();
-      const uint32_t trow = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
-                            static_cast<uint32_t>(acc * BN);
-      const int64_t grow = static_cast<int64_t>(t.row0) + r_in_tile;
-      const bool row_ok = r_in_tile < nrows;
-      const bool quad_full = (quad + 1) * 32 <= nrows;
-      constexpr int kChunks = SWIGLU ? BN / 64 : BN / 32;  // of 32 output columns
-      if (quad * 32 < nrows) {
-#pragma unroll 1
-        for (int c = half; c < kChunks; c += 2) {
-          const int col0 = (t.n * kChunks + c) * 32;
-          if (col0 >= p.N) break;
-          float v[32];
-          load_chunk<SWIGLU>(trow + (SWIGLU ? 64 : 32) * c, v);
-          store_chunk<QOUT>(v, p, &tmC, col0, grow, t.row0 + quad * 32, row_ok, quad_full, stg);
-        }
-      }
+      epilogue_tile<SWIGLU, QOUT>(p, &tmC, w, tmem_base + acc.slot * kAccCols, t.row0,
+                                  min(MM, t.row_end - t.row0), t.c0, t.nc, stg);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&ctl.acc_empty[acc]));
-      if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
+      if (lane == 0) mbar_arrive(smem_u32(&ctl.acc_empty[acc.slot]));
+      acc.next(kAccs);
     }
     if (lane == 0) bulk_wait_group_all();
     __syncwarp();
@@ -335,16 +331,17 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-template <int BN, bool SWIGLU, bool QOUT>
+template <bool SWIGLU, bool QOUT>
 cudaError_t launch_variant(unsigned grid, const CUtensorMap& ma, const CUtensorMap& mb,
-                           const CUtensorMap& mc, const Params& p, cudaStream_t st) {
+                           const CUtensorMap& mr, const CUtensorMap& mc, const Params& p,
+                           cudaStream_t st) {
   static int done[64] = {0};
   static std::mutex mu;
   const cudaError_t e =
-      allow_smem(grouped_gemm_mxfp4_kernel<BN, SWIGLU, QOUT>, smem_bytes<BN>(), done, mu);
+      allow_smem(grouped_gemm_mxfp4_kernel<SWIGLU, QOUT>, kSmemBytes, done, mu);
   if (e != cudaSuccess) return e;
-  return launch_pdl(kPdlGemm, grouped_gemm_mxfp4_kernel<BN, SWIGLU, QOUT>, dim3(grid),
-                    dim3(kThreads), smem_bytes<BN>(), st, ma, mb, mc, p);
+  return launch_pdl(kPdlGemm, grouped_gemm_mxfp4_kernel<SWIGLU, QOUT>, dim3(grid), dim3(kThreads),
+                    kSmemBytes, st, ma, mb, mr, mc, p);
 }
 
 }  // namespace
@@ -363,18 +360,6 @@ bool make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool make_scale_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t nkb) {
-  EncodeTiledFn enc = encode_fn();
-  if (!enc) return false;
-  const cuuint64_t dims[3] = {256, nkb, rows};
-  const cuuint64_t strides[2] = {1024, 1024 * nkb};
-  const cuuint32_t box[3] = {256, 1, 2};
-  const cuuint32_t estr[3] = {1, 1, 1};
-  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), dims, strides, box,
-             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 }  // namespace mx
 
 cudaError_t launch_grouped_gemm_mxfp4(const MxGemmArgs& a, cudaStream_t st) {
@@ -384,25 +369,24 @@ cudaError_t launch_grouped_gemm_mxfp4(const MxGemmArgs& a, cudaStream_t st) {
   const int forced = forced_gemm_kernel();
   if (forced >= 0 ? forced == 1 : a.M > 192 * static_cast<int64_t>(a.G))
     return launch_grouped_gemm_mxfp4_pair(a, st);
-  constexpr int BN = 128;
   Params p = make_params(a);
   p.a_box_rows = a.M > 64 * static_cast<int64_t>(a.G) ? 128 : 32;
-  p.n_tiles = cdiv(p.b_rows, BN);
   const uint64_t cb = static_cast<uint64_t>(mx_code_bytes(a.K));
-  CUtensorMap ma, mb, mc;
+  CUtensorMap ma, mb, mr, mc;
   if (!make_code_map(&ma, a.rows, static_cast<uint64_t>(a.M), cb, p.a_row_bytes, p.a_box_rows) ||
-      !make_code_map(&mb, a.weight, static_cast<uint64_t>(a.G) * p.b_rows, cb, cb, BN))
+      !make_raw_map(&mr, a.rows, static_cast<uint64_t>(a.M), p.a_row_bytes, p.a_box_rows) ||
+      !make_code_map(&mb, a.weight, static_cast<uint64_t>(a.G) * p.b_rows, cb, cb, 64))
     return cudaErrorInvalidValue;
   if (a.quantized_out)
     mc = ma;  // not used
   else if (!make_out_map(&mc, a.out, static_cast<uint64_t>(a.M), static_cast<uint64_t>(a.N)))
     return cudaErrorInvalidValue;
   const int sms = num_sms_for_current_device();
-  const int64_t max_tiles = (cdiv64(a.M, MM) + a.G) * p.n_tiles;
+  const int64_t max_tiles = (cdiv64(a.M, MM) + a.G) * p.ct.tiles;
   const unsigned grid = static_cast<unsigned>(max_tiles < sms ? max_tiles : sms);
-  if (!a.swiglu) return launch_variant<BN, false, false>(grid, ma, mb, mc, p, st);
-  if (a.quantized_out) return launch_variant<BN, true, true>(grid, ma, mb, mc, p, st);
-  return launch_variant<BN, true, false>(grid, ma, mb, mc, p, st);
+  if (!a.swiglu) return launch_variant<false, false>(grid, ma, mb, mr, mc, p, st);
+  if (a.quantized_out) return launch_variant<true, true>(grid, ma, mb, mr, mc, p, st);
+  return launch_variant<true, false>(grid, ma, mb, mr, mc, p, st);
 }
 
 }  // namespace hmoe

@@ -17,6 +17,13 @@ constexpr int kMaxGroups = 1024;
 constexpr int kAtom = 512;   // scales of 128 rows x 128 elements
 constexpr int kEpiBox = 32 * 32 * 2;
 constexpr int kTmemCols = 512;
+constexpr int kAccCols = 64 * kMxTileChunks;
+constexpr int kAccs = 2;
+constexpr int kEpiWarps = 12;  // three per lane quadrant
+constexpr int kThreads = 128 + 32 * kEpiWarps;
+constexpr int kSfaCols = 8;                  // TMEM columns of a k-block's scales
+constexpr int kSfbCols = 4 * kMxTileChunks;
+constexpr int kSfbBytes = kMxTileChunks * kAtom;
 
 struct Params {
   const uint8_t* a_rows;    // records
@@ -28,11 +35,9 @@ struct Params {
   int K;
   int a_row_bytes;
   int a_box_rows;   // rows of one A load (single-CTA kernel)
-  int n_tiles;
-  int tile_chunks;  // 64-column chunks of a column tile (pair kernel); the first
-  int tile_extra;   // tile_extra tiles have one more
+  MxColTiles ct;    // column tiles
   int b_rows;       // packed rows per group
-  int b_chunks;     // 128-row scale chunks per group
+  int b_chunks;     // 64-row chunks per group
   void* out;        // bf16 [M, N] or records
   int* err;
   unsigned long long wait_limit_ns;
@@ -111,6 +116,15 @@ __device__ __forceinline__ void st_shared_v4m(uint32_t addr, uint4 v) {
                "r"(v.w)
                : "memory");
 }
+
+// A place in a ring of barriers, and the parity of its phase.
+struct Ring {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int size) {
+    if (++slot == size) { slot = 0; phase ^= 1u; }
+  }
+};
 
 struct GroupTables {
   int group_rows[kMaxGroups + 1];
@@ -250,7 +264,8 @@ __device__ __forceinline__ void store_chunk(const float (&v)[32], const Params& 
 }
 
 // 32 output columns out of TMEM: 32 accumulator columns, or (SWIGLU) the 32
-// gate columns and the 32 up columns behind them.
+// gate columns and the 32 up columns behind them.  The wait names the
+// registers, so that no use of them can move above it.
 template <bool SWIGLU>
 __device__ __forceinline__ void load_chunk(uint32_t taddr, float (&v)[32]) {
   uint32_t ra[32];
@@ -258,13 +273,36 @@ __device__ __forceinline__ void load_chunk(uint32_t taddr, float (&v)[32]) {
   if constexpr (SWIGLU) {
     uint32_t ua[32];
     tmem_ld_32cols(taddr + 32, ua);
-    tc_wait_ld();
+    tc_wait_ld_regs(ra);
+    tc_wait_ld_regs(ua);
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = silu_mul(__uint_as_float(ra[i]), __uint_as_float(ua[i]));
   } else {
-    tc_wait_ld();
+    tc_wait_ld_regs(ra);
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(ra[i]);
+  }
+}
+
+// One CTA's 128 rows of a finished tile, for epilogue warp `w` of kEpiWarps
+// (row quadrant = warp index mod 4; three warps share a quadrant's columns).
+template <bool SWIGLU, bool QOUT>
+__device__ __forceinline__ void epilogue_tile(const Params& p, const CUtensorMap* tmC, int w,
+                                              uint32_t acc_tmem, int row0, int nrows, int chunk0,
+                                              int chunks, uint32_t stg) {
+  const int quad = w & 3, third = w >> 2;
+  if (quad * 32 >= nrows) return;
+  const int lane = threadIdx.x & 31;
+  const int r = quad * 32 + lane;
+  constexpr int kPer = SWIGLU ? 1 : 2;  // 32-column outputs of a chunk
+#pragma unroll 1
+  for (int c = third; c < chunks * kPer; c += kEpiWarps / 4) {
+    const int col0 = (chunk0 * kPer + c) * 32;
+    if (col0 >= p.N) break;
+    float v[32];
+    load_chunk<SWIGLU>(acc_tmem + (static_cast<uint32_t>(quad * 32) << 16) + (SWIGLU ? 64 : 32) * c, v);
+    store_chunk<QOUT>(v, p, tmC, col0, static_cast<int64_t>(row0) + r, row0 + quad * 32, r < nrows,
+                      (quad + 1) * 32 <= nrows, stg);
   }
 }
 
@@ -272,13 +310,22 @@ __device__ __forceinline__ void load_chunk(uint32_t taddr, float (&v)[32]) {
 bool make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t rows,
               uint64_t cols, uint64_t stride, uint32_t box_rows, uint32_t box_cols,
               CUtensorMapSwizzle swizzle);
-// Scale chunks of 1024 bytes [rows][nkb]: boxes of two rows' chunks of one k-block.
-bool make_scale_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t nkb);
 // Codes [rows, cols bytes] with a row stride, boxes of box_rows x 128 bytes.
 inline bool make_code_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
                           uint64_t stride, uint32_t box_rows) {
   return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rows, cols, stride, box_rows, kRowB,
                   CU_TENSOR_MAP_SWIZZLE_128B);
+}
+// Whole records, boxes of box_rows x 16 bytes (the scales of two k-blocks).
+inline bool make_raw_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t row_bytes,
+                         uint32_t box_rows) {
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rows, row_bytes, row_bytes, box_rows, 16,
+                  CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+// Scale atoms of 512 bytes, boxes of several.
+inline bool make_scale_map(CUtensorMap* map, const void* base, uint64_t atoms, uint32_t box) {
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, atoms, 128, 512, box, 128,
+                  CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 inline bool make_out_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols) {
   return make_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, rows, cols, cols * 2, 32, 32,
@@ -297,8 +344,8 @@ inline Params make_params(const MxGemmArgs& a) {
   p.a_row_bytes = mx_row_bytes(a.K);
   p.a_box_rows = MM;
   p.b_rows = mx_weight_rows(a.N, a.swiglu);
-  p.b_chunks = cdiv(p.b_rows, 128);
-  p.n_tiles = p.tile_chunks = p.tile_extra = 0;
+  p.b_chunks = cdiv(p.b_rows, 64);
+  p.ct = mx_col_tiles(p.b_rows);
   p.out = a.out;
   p.err = a.err;
   p.wait_limit_ns = kWaitLimitNs;

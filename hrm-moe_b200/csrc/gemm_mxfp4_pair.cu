@@ -15,14 +15,13 @@
 // XL gate_up at T=16384: 0.54 GB of operands to the SMs instead of 0.86 GB.
 //
 // TMEM (512 columns): two 192-column accumulators, six slots of A scales
-// (8 columns), five of B scales (16).  192 columns rather than 256: two
+// (8 columns) and of B scales (12).  192 columns rather than 256: two
 // accumulators of 256 would leave no column for the scales.  A slot's scales
 // live as long as its codes, under the same barriers.
 //
-// Column tiles are runs of 64-column chunks, balanced (16 chunks: 3, 3, 3, 3,
-// 2, 2).  The row blocks of all groups, each split into `parts` runs of
-// column tiles, are the units the pairs take in turn; parts is the count that
-// gives the shortest schedule for the actual row counts, found on the device.
+// The row blocks of all groups, each split into `parts` runs of column tiles,
+// are the units the pairs take in turn; parts is the count that gives the
+// shortest schedule for the actual row counts, found on the device.
 #include "gemm_mxfp4.cuh"
 
 namespace hmoe {
@@ -30,23 +29,21 @@ namespace mx {
 namespace {
 
 constexpr int QA = 6;             // k-blocks of A
-constexpr int QB = 5;             // k-blocks of B
-constexpr int kTileChunks = 3;    // 64-column chunks of a tile
-constexpr int kAccCols = 64 * kTileChunks;
-constexpr int kAccs = 2;
+constexpr int QB = 6;             // k-blocks of B
+constexpr int QR = 3;             // pairs of k-blocks of A's scales: as they come, and as atoms
 constexpr int kABytes = MM * kRowB;
 constexpr int kBChunkBytes = 32 * kRowB;  // a CTA's half of a chunk
-constexpr int kBBytes = kTileChunks * kBChunkBytes;
-constexpr int kEpiWarps = 12;
-constexpr int kThreads = 128 + 32 * kEpiWarps;
+constexpr int kBBytes = kMxTileChunks * kBChunkBytes;
 constexpr int kSfaCol = kAccs * kAccCols;
-constexpr int kSfbCol = kSfaCol + 8 * QA;
-static_assert(kSfbCol + 16 * QB <= kTmemCols, "TMEM columns");
+constexpr int kSfbCol = kSfaCol + kSfaCols * QA;
+static_assert(kSfbCol + kSfbCols * QB <= kTmemCols, "TMEM columns");
 
 struct Ctl {
   uint64_t a_full[QA], a_empty[QA];
   uint64_t b_full[QB], b_empty[QB];
   uint64_t sf_full[QB];  // the k-block's scales are in TMEM
+  uint64_t raw_full[QR], raw_empty[QR];
+  uint64_t sfa_full[QR], sfa_empty[QR];
   uint64_t acc_full[kAccs], acc_empty[kAccs];
   uint64_t drain;
   uint32_t tmem_base;
@@ -56,9 +53,10 @@ struct Ctl {
 };
 
 constexpr int kOffSfa = QA * kABytes;
-constexpr int kOffB = kOffSfa + QA * 1024;
+constexpr int kOffB = kOffSfa + QR * 2048;
 constexpr int kOffSfb = kOffB + QB * kBBytes;
-constexpr int kOffEpi = kOffSfb + QB * 2048;
+constexpr int kOffRaw = kOffSfb + QB * kSfbBytes;  // [128 rows][16 scales]
+constexpr int kOffEpi = kOffRaw + QR * 2048;
 constexpr int kOffCtl = kOffEpi + kEpiWarps * kEpiBox;
 constexpr size_t kSmemBytes = 1024 + kOffCtl + sizeof(Ctl);
 static_assert(kSmemBytes <= 232448, "shared memory budget of one sm_100 CTA");
@@ -97,14 +95,6 @@ __device__ __forceinline__ bool wait_cluster_bounded(uint32_t bar, uint32_t pari
   }
 }
 
-struct Ring {
-  int slot = 0;
-  uint32_t phase = 0;
-  __device__ __forceinline__ void next(int size) {
-    if (++slot == size) { slot = 0; phase ^= 1u; }
-  }
-};
-
 // A unit: a row block and its column tiles [t0, t1).
 struct Unit : RowBlock {
   int t0, t1;
@@ -117,22 +107,6 @@ __device__ __forceinline__ Unit find_unit(const Ctl& ctl, int G, int n_tiles, in
   r.t0 = part * n_tiles / ctl.parts;
   r.t1 = (part + 1) * n_tiles / ctl.parts;
   return r;
-}
-// Column tile t: its first 64-column chunk and its number of chunks.
-struct ColTile {
-  int c0, nc;
-};
-__device__ __forceinline__ ColTile col_tile(const Params& p, int t) {
-  return ColTile{t * p.tile_chunks + min(t, p.tile_extra), p.tile_chunks + (t < p.tile_extra)};
-}
-
-__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1,
-                                                 int c2, uint32_t bar_cluster) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar_cluster)
-      : "memory");
 }
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int c0, int c1) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(
@@ -147,6 +121,8 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
                                const __grid_constant__ CUtensorMap tmB,
                                const __grid_constant__ CUtensorMap tmB1,
                                const __grid_constant__ CUtensorMap tmS,
+                               const __grid_constant__ CUtensorMap tmS1,
+                               const __grid_constant__ CUtensorMap tmR,
                                const __grid_constant__ CUtensorMap tmC, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -164,13 +140,19 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
   if (warp == 0) {
     if (lane == 0) {
       for (int s = 0; s < QA; ++s) {
-        mbar_init(smem_u32(&ctl.a_full[s]), 3);   // the leader's arm, both CTAs' scale warps
+        mbar_init(smem_u32(&ctl.a_full[s]), 1);   // the leader's arm
         mbar_init(smem_u32(&ctl.a_empty[s]), 1);  // one commit per use
       }
       for (int s = 0; s < QB; ++s) {
         mbar_init(smem_u32(&ctl.b_full[s]), 1);
         mbar_init(smem_u32(&ctl.b_empty[s]), 1);
         mbar_init(smem_u32(&ctl.sf_full[s]), 1);
+      }
+      for (int s = 0; s < QR; ++s) {
+        mbar_init(smem_u32(&ctl.raw_full[s]), 1);
+        mbar_init(smem_u32(&ctl.raw_empty[s]), 1);
+        mbar_init(smem_u32(&ctl.sfa_full[s]), 2);   // both CTAs' scale warps
+        mbar_init(smem_u32(&ctl.sfa_empty[s]), 1);
       }
       for (int a = 0; a < kAccs; ++a) {
         mbar_init(smem_u32(&ctl.acc_full[a]), 1);
@@ -183,6 +165,8 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
       tma_prefetch_desc(&tmB);
       tma_prefetch_desc(&tmB1);
       tma_prefetch_desc(&tmS);
+      tma_prefetch_desc(&tmS1);
+      tma_prefetch_desc(&tmR);
       tma_prefetch_desc(&tmC);
     }
     __syncwarp();
@@ -195,9 +179,9 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
       const int mt = ctl.tab.num_m_tiles;
       int best = 1;
       int64_t best_cost = INT64_MAX;
-      for (int parts = 1; parts <= min(p.n_tiles, 64); ++parts) {
+      for (int parts = 1; parts <= min(p.ct.tiles, 64); ++parts) {
         const int64_t cost = cdiv64(static_cast<int64_t>(mt) * parts, npairs) *
-                             (8 * cdiv(p.n_tiles, parts) + 1);
+                             (8 * cdiv(p.ct.tiles, parts) + 1);
         if (cost < best_cost) { best_cost = cost; best = parts; }
       }
       ctl.parts = best;
@@ -212,7 +196,7 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
   grid_dependency_wait();
   grid_launch_dependents();
 
-  const uint32_t tmem_base = ctl.tmem_base;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl.tmem_base, 0);  // uniform, and seen to be
   const int units = ctl.tab.num_m_tiles * ctl.parts;
   const int kp = mx_padded_k(p.K);
   const int nkb = cdiv(kp, kMxKBlock);
@@ -224,28 +208,38 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (elect_one()) {
-      Ring a, b;
+      Ring a, b, raw;
       bool ok = true;
+      const int soff = mx_code_bytes(p.K);
+      // A's scales of k-blocks kb and kb + 1, as the records hold them
+      auto load_raw = [&](int row0, int kb) {
+        if (!mbar_wait_bounded(smem_u32(&ctl.raw_empty[raw.slot]), raw.phase ^ 1u, abort, p.err, lim))
+          return false;
+        const uint32_t fb = smem_u32(&ctl.raw_full[raw.slot]);
+        mbar_arrive_expect_tx(fb, 2048);
+        tma_load_2d(sbase + kOffRaw + raw.slot * 2048, &tmR, soff + kb * 8, row0, fb);
+        raw.next(QR);
+        return true;
+      };
+      Unit un, next;
+      if (pair < units) next = find_unit(ctl, G, p.ct.tiles, pair);
+      if (resident && pair < units)
+        for (int kb = 0; ok && kb < nkb; kb += 2) ok = load_raw(next.row0 + static_cast<int>(rank) * MM, kb);
       for (int u = pair; ok && u < units; u += npairs) {
-        const Unit un = find_unit(ctl, G, p.n_tiles, u);
+        un = next;
         const int my_row0 = un.row0 + static_cast<int>(rank) * MM;
-        // the next unit's A into L2: its loads come in one burst from every
-        // pair as this unit's last tile ends
-        if (resident && u + npairs < units) {
-          const int next_row0 =
-              find_unit(ctl, G, p.n_tiles, u + npairs).row0 + static_cast<int>(rank) * MM;
-          for (int kb = 0; kb < nkb; ++kb) tma_prefetch_2d(&tmA, kb * kRowB, next_row0);
-        }
         for (int t = un.t0; ok && t < un.t1; ++t) {
-          const ColTile ct = col_tile(p, t);
-          const CUtensorMap* mapB = t < p.tile_extra ? &tmB1 : &tmB;
-          const int brow = un.g * p.b_rows + ct.c0 * 64 + static_cast<int>(rank) * ct.nc * 32;
-          const int srow = un.g * p.b_chunks + (ct.c0 >> 1);
-          const uint32_t bytes = 2 * (ct.nc * kBChunkBytes + 2048);  // both CTAs'
+          const bool longer = t < p.ct.extra;
+          const CUtensorMap *mapB = longer ? &tmB1 : &tmB, *mapS = longer ? &tmS1 : &tmS;
+          const int c0 = p.ct.first(t), nc = p.ct.count(t);
+          const int brow = un.g * p.b_rows + c0 * 64 + static_cast<int>(rank) * nc * 32;
+          const int srow = (un.g * p.b_chunks + c0) * nkb;
+          const uint32_t bytes = 2 * nc * (kBChunkBytes + kAtom);  // both CTAs'
           const bool load_a = t == un.t0 || !resident;
           for (int kb = 0; kb < nkb; ++kb) {
             if (load_a) {
-              if (!mbar_wait_bounded(smem_u32(&ctl.a_empty[a.slot]), a.phase ^ 1u, abort, p.err, lim)) {
+              if ((!resident && (kb & 1) == 0 && !load_raw(my_row0, kb)) ||
+                  !mbar_wait_bounded(smem_u32(&ctl.a_empty[a.slot]), a.phase ^ 1u, abort, p.err, lim)) {
                 ok = false;
                 break;
               }
@@ -263,8 +257,20 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
             const uint32_t fb_leader = map_to_rank(fb, 0);
             if (leader) mbar_arrive_expect_tx(fb, bytes);
             tma_load_2d_pair(sbase + kOffB + b.slot * kBBytes, mapB, kb * kRowB, brow, fb_leader);
-            tma_load_3d_pair(sbase + kOffSfb + b.slot * 2048, &tmS, 0, kb, srow, fb_leader);
+            tma_load_2d_pair(sbase + kOffSfb + b.slot * kSfbBytes, mapS, 0, srow + kb * nc, fb_leader);
             b.next(QB);
+          }
+          if (ok && t == un.t0 && u + npairs < units) {
+            // the next unit: its scales into the raw ring, its codes into L2
+            // (the loads come in one burst, from every pair, as this unit's
+            // last tile ends)
+            next = find_unit(ctl, G, p.ct.tiles, u + npairs);
+            const int row0 = next.row0 + static_cast<int>(rank) * MM;
+            if (resident)
+              for (int kb = 0; ok && kb < nkb; ++kb) {
+                if ((kb & 1) == 0) ok = load_raw(row0, kb);
+                tma_prefetch_2d(&tmA, kb * kRowB, row0);
+              }
           }
         }
       }
@@ -274,6 +280,8 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
         if (!mbar_wait_bounded(smem_u32(&ctl.a_empty[a.slot]), a.phase ^ 1u, &never, p.err, lim)) break;
       for (int i = 0; i < QB; ++i, b.next(QB))
         if (!mbar_wait_bounded(smem_u32(&ctl.b_empty[b.slot]), b.phase ^ 1u, &never, p.err, lim)) break;
+      for (int i = 0; i < QR; ++i, raw.next(QR))
+        if (!mbar_wait_bounded(smem_u32(&ctl.raw_empty[raw.slot]), raw.phase ^ 1u, &never, p.err, lim)) break;
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
@@ -282,15 +290,13 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
       bool ok = true;
       const uint64_t adesc0 = smem_desc_sw128(sbase), bdesc0 = smem_desc_sw128(sbase + kOffB);
       for (int u = pair; ok && u < units; u += npairs) {
-        const Unit un = find_unit(ctl, G, p.n_tiles, u);
+        const Unit un = find_unit(ctl, G, p.ct.tiles, u);
         const int first = a.slot;  // the row block's first slot (resident)
         for (int t = un.t0; ok && t < un.t1; ++t) {
-          const ColTile ct = col_tile(p, t);
+          const int nc = p.ct.count(t);
           const bool load_a = t == un.t0 || !resident;
           const bool free_a = t == un.t1 - 1 || !resident;
-          const uint32_t id0 = idesc_mxf4(2 * MM, 64 * ct.nc, 0), id1 = idesc_mxf4(2 * MM, 64 * ct.nc, 2);
-          // a tile that starts in the middle of a scale atom: two columns in
-          const uint32_t sfb0 = tmem_base + kSfbCol + 2 * (ct.c0 & 1);
+          const uint32_t id0 = idesc_mxf4(2 * MM, 64 * nc, 0), id1 = idesc_mxf4(2 * MM, 64 * nc, 2);
           if (!mbar_wait_bounded(smem_u32(&ctl.acc_empty[acc.slot]), acc.phase ^ 1u, abort, p.err, lim)) {
             ok = false;
             break;
@@ -301,26 +307,23 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
           for (int kb = 0; kb < nkb; ++kb) {
             if (load_a) {
               sa = a.slot;
-              if (!wait_cluster_bounded(smem_u32(&ctl.a_full[sa]), a.phase, abort, p.err, lim)) {
-                ok = false;
-                break;
-              }
               a.next(QA);
             }
-            if (!mbar_wait_bounded(smem_u32(&ctl.b_full[b.slot]), b.phase, abort, p.err, lim) ||
-                !mbar_wait_bounded(smem_u32(&ctl.sf_full[b.slot]), b.phase, abort, p.err, lim)) {
+            // committed by a thread that has waited for the k-block's A and B
+            if (!mbar_wait_bounded(smem_u32(&ctl.sf_full[b.slot]), b.phase, abort, p.err, lim)) {
               ok = false;
               break;
             }
             tc_fence_after();
             const uint64_t ad = adesc0 + sa * (kABytes >> 4), bd = bdesc0 + b.slot * (kBBytes >> 4);
-            const uint32_t tsfa = tmem_base + kSfaCol + 8 * sa, tsfb = sfb0 + 16 * b.slot;
+            const uint32_t tsfa = tmem_base + kSfaCol + kSfaCols * sa;
+            const uint32_t tsfb = tmem_base + kSfbCol + kSfbCols * b.slot;
             const int mmas = min(4, cdiv(kp - kb * kMxKBlock, 64));
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
               if (kk >= mmas) break;
               mma_mxf4_pair(d_tmem, ad + 2 * kk, bd + 2 * kk, (kk & 1) ? id1 : id0,
-                            tsfa + 4 * (kk >> 1), tsfb + 8 * (kk >> 1), (kb | kk) != 0 ? 1u : 0u);
+                            tsfa + 4 * (kk >> 1), tsfb + 2 * nc * (kk >> 1), (kb | kk) != 0 ? 1u : 0u);
             }
             tc_commit_pair_both(smem_u32(&ctl.b_empty[b.slot]));
             b.next(QB);
@@ -342,47 +345,49 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
     }
   } else if (warp == 3) {
     // ------------------------------------------- scales from shared memory to TMEM
-    // A thread of its own: the copies of the next k-blocks run, and are
-    // issued, beside this one's MMAs (in the MMA thread they took longer to
-    // issue than the MMAs, 154 -> 138 us for XL gate_up with everything else
-    // as it is).  The MMA thread waits for them through sf_full; b_full and
-    // a_full, which it waits for too, order the slot's reuse.
+    // A thread of its own: each tcgen05 instruction takes 40 to 65 cycles to
+    // issue, and copies and MMAs in one thread took longer to issue than the
+    // MMAs to run.  sf_full (commit, mbarrier, fence) hands a k-block on to the
+    // MMA thread.
     if (leader && elect_one()) {
-      Ring a, b;
+      Ring a, sa, b;
       bool ok = true;
       const uint64_t sfa0 = smem_desc_atom(sbase + kOffSfa), sfb0 = smem_desc_atom(sbase + kOffSfb);
       for (int u = pair; ok && u < units; u += npairs) {
-        const Unit un = find_unit(ctl, G, p.n_tiles, u);
+        const Unit un = find_unit(ctl, G, p.ct.tiles, u);
         for (int t = un.t0; ok && t < un.t1; ++t) {
-          const ColTile ct = col_tile(p, t);
+          const int nc = p.ct.count(t);
           const bool load_a = t == un.t0 || !resident;
-          const bool two = (ct.c0 & 1) + ct.nc > 2;  // atoms of 128 rows that the tile reaches
           for (int kb = 0; kb < nkb; ++kb) {
             if (load_a) {
-              if (!wait_cluster_bounded(smem_u32(&ctl.a_full[a.slot]), a.phase, abort, p.err, lim)) {
+              // a_full: the slot's TMEM columns are free as its codes are
+              if (((kb & 1) == 0 && !wait_cluster_bounded(smem_u32(&ctl.sfa_full[sa.slot]), sa.phase,
+                                                          abort, p.err, lim)) ||
+                  !mbar_wait_bounded(smem_u32(&ctl.a_full[a.slot]), a.phase, abort, p.err, lim)) {
                 ok = false;
                 break;
               }
               tc_fence_after();
-              const uint32_t tsfa = tmem_base + kSfaCol + 8 * a.slot;
-              const uint64_t d = sfa0 + a.slot * (1024 >> 4);
+              const uint32_t tsfa = tmem_base + kSfaCol + kSfaCols * a.slot;
+              const uint64_t d = sfa0 + ((sa.slot * 2048 + (kb & 1) * 1024) >> 4);
               tmem_cp_atom_pair(tsfa, d);
               tmem_cp_atom_pair(tsfa + 4, d + (kAtom >> 4));
               a.next(QA);
+              if ((kb & 1) != 0 || kb == nkb - 1) {
+                tc_commit_pair_both(smem_u32(&ctl.sfa_empty[sa.slot]));
+                sa.next(QR);
+              }
             }
             if (!mbar_wait_bounded(smem_u32(&ctl.b_full[b.slot]), b.phase, abort, p.err, lim)) {
               ok = false;
               break;
             }
             tc_fence_after();
-            const uint32_t tsfb = tmem_base + kSfbCol + 16 * b.slot;
-            const uint64_t d = sfb0 + b.slot * (2048 >> 4);
-            tmem_cp_atom_pair(tsfb, d);
-            tmem_cp_atom_pair(tsfb + 8, d + (kAtom >> 4));
-            if (two) {
-              tmem_cp_atom_pair(tsfb + 4, d + (1024 >> 4));
-              tmem_cp_atom_pair(tsfb + 12, d + ((1024 + kAtom) >> 4));
-            }
+            const uint32_t tsfb = tmem_base + kSfbCol + kSfbCols * b.slot;
+            const uint64_t d = sfb0 + b.slot * (kSfbBytes >> 4);
+#pragma unroll
+            for (int c = 0; c < kMxTileChunks; ++c)
+              if (c < nc) tmem_cp_atom_pair(tsfb + 4 * c, d + c * (kAtom >> 4));
             tc_commit_pair(smem_u32(&ctl.sf_full[b.slot]));
             b.next(QB);
           }
@@ -391,103 +396,70 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
     }
   } else if (warp == 2) {
     // ------------------------------------------------------ scales of A
-    // Lane i brings this CTA's rows i, i + 32, i + 64, i + 96: batches of four
-    // k-blocks, the next batch's loads in flight while this one is stored.
-    const int r0 = static_cast<int>(rank) * MM + lane;
-    const int soff = mx_code_bytes(p.K);
-    Ring a;
-    uint2 cur[4][4], nxt[4][4];
-    auto load = [&](const Unit& un, int kb0, uint2 (&v)[4][4]) {
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const int row = un.row0 + r0 + 32 * h;
-        const uint8_t* src = p.a_rows + static_cast<int64_t>(row) * p.a_row_bytes + soff;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v[h][i] = row < un.row_end && kb0 + i < nkb
-                        ? *reinterpret_cast<const uint2*>(src + (kb0 + i) * 8)
-                        : make_uint2(0, 0);
-      }
-    };
-    int u = pair, kb0 = 0, t = 0;
-    Unit un;
+    // From the records' order into the atoms': lane i moves this CTA's rows
+    // i, i + 32, i + 64, i + 96, whose words make up one lane of an atom.  Two
+    // k-blocks at a time, ahead of the codes: the release at cluster scope
+    // takes about 900 cycles.  (Loading the scales straight from global memory
+    // was slower: the proxy fence waits for the loads in flight behind it.)
+    Ring raw, sa;
     bool ok = true;
-    if (u < units) {
-      un = find_unit(ctl, G, p.n_tiles, u);
-      t = un.t0;
-      load(un, 0, cur);
-    }
-    while (ok && u < units) {
-      int nkb0 = kb0 + 4;
-      if (nkb0 >= nkb) {
-        nkb0 = 0;
-        t = resident ? un.t1 : t + 1;
-        if (t >= un.t1) {
-          u += npairs;
-          if (u < units) {
-            un = find_unit(ctl, G, p.n_tiles, u);
-            t = un.t0;
-          }
-        }
+    for (int u = pair; ok && u < units; u += npairs) {
+      int reps = 1;  // how often the unit's A is loaded
+      if (!resident) {
+        const Unit un = find_unit(ctl, G, p.ct.tiles, u);
+        reps = un.t1 - un.t0;
       }
-      if (u < units) load(un, nkb0, nxt);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (kb0 + i >= nkb) break;
-        if (!mbar_wait_bounded(smem_u32(&ctl.a_empty[a.slot]), a.phase ^ 1u, abort, p.err, lim)) {
+      for (int i = 0; ok && i < reps * cdiv(nkb, 2); ++i) {
+        if (!mbar_wait_bounded(smem_u32(&ctl.raw_full[raw.slot]), raw.phase, abort, p.err, lim)) {
           ok = false;
           break;
         }
-        const uint32_t dst = sbase + kOffSfa + a.slot * 1024 + lane * 16;
-        // the atom's 16 bytes of a lane: its four rows' words
-        st_shared_v4m(dst, make_uint4(cur[0][i].x, cur[1][i].x, cur[2][i].x, cur[3][i].x));
-        st_shared_v4m(dst + kAtom, make_uint4(cur[0][i].y, cur[1][i].y, cur[2][i].y, cur[3][i].y));
+        const uint4* src = reinterpret_cast<const uint4*>(smem + kOffRaw + raw.slot * 2048) + lane;
+        uint4 v[4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) v[h] = src[32 * h];
+        if (!mbar_wait_bounded(smem_u32(&ctl.sfa_empty[sa.slot]), sa.phase ^ 1u, abort, p.err, lim)) {
+          ok = false;
+          break;
+        }
+        const uint32_t dst = sbase + kOffSfa + sa.slot * 2048 + lane * 16;
+        st_shared_v4m(dst, make_uint4(v[0].x, v[1].x, v[2].x, v[3].x));
+        st_shared_v4m(dst + kAtom, make_uint4(v[0].y, v[1].y, v[2].y, v[3].y));
+        st_shared_v4m(dst + 1024, make_uint4(v[0].z, v[1].z, v[2].z, v[3].z));
+        st_shared_v4m(dst + 1024 + kAtom, make_uint4(v[0].w, v[1].w, v[2].w, v[3].w));
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) arrive_release_cluster(map_to_rank(smem_u32(&ctl.a_full[a.slot]), 0));
-        a.next(QA);
+        // only here: the stores have taken the values, so the loads are done
+        // (an arrival right behind the loads let the next copy overtake them)
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&ctl.raw_empty[raw.slot]));
+          arrive_release_cluster(map_to_rank(smem_u32(&ctl.sfa_full[sa.slot]), 0));
+        }
+        raw.next(QR);
+        sa.next(QR);
       }
-#pragma unroll
-      for (int h = 0; h < 4; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) cur[h][i] = nxt[h][i];
-      kb0 = nkb0;
     }
-  } else {
+    // no commit is on its way to this CTA's barriers when it leaves
+    for (int i = 0; i < QR; ++i, sa.next(QR))
+      if (!mbar_wait_bounded(smem_u32(&ctl.sfa_empty[sa.slot]), sa.phase ^ 1u, &never, p.err, lim)) break;
+  } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
-    const int quad = warp & 3;
-    const int third = (warp - 4) >> 2;
-    const int r_in_tile = quad * 32 + lane;
-    const uint32_t stg = sbase + kOffEpi + (warp - 4) * kEpiBox;
+    const int w = warp - 4;
+    const uint32_t stg = sbase + kOffEpi + w * kEpiBox;
     Ring acc;
     bool ok = true;
     for (int u = pair; ok && u < units; u += npairs) {
-      const Unit un = find_unit(ctl, G, p.n_tiles, u);
+      const Unit un = find_unit(ctl, G, p.ct.tiles, u);
       const int my_row0 = un.row0 + static_cast<int>(rank) * MM;
       const int nrows = min(MM, un.row_end - my_row0);  // may be <= 0: nothing to store
-      const int64_t grow = static_cast<int64_t>(my_row0) + r_in_tile;
-      const bool row_ok = r_in_tile < nrows;
-      const bool quad_full = (quad + 1) * 32 <= nrows;
       for (int t = un.t0; t < un.t1; ++t) {
-        const ColTile ct = col_tile(p, t);
         if (!mbar_wait_bounded(smem_u32(&ctl.acc_full[acc.slot]), acc.phase, abort, p.err, lim)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t trow = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) +
-                              static_cast<uint32_t>(acc.slot * kAccCols);
-        constexpr int kPer = SWIGLU ? 1 : 2;  // 32-column outputs of a chunk
-        if (quad * 32 < nrows) {
-#pragma unroll 1
-          for (int c = third; c < ct.nc * kPer; c += 3) {
-            const int col0 = (ct.c0 * kPer + c) * 32;
-            if (col0 >= p.N) break;
-            float v[32];
-            load_chunk<SWIGLU>(trow + (SWIGLU ? 64 : 32) * c, v);
-            store_chunk<QOUT>(v, p, &tmC, col0, grow, my_row0 + quad * 32, row_ok, quad_full, stg);
-          }
-        }
+        epilogue_tile<SWIGLU, QOUT>(p, &tmC, w, tmem_base + acc.slot * kAccCols, my_row0, nrows,
+                                    p.ct.first(t), p.ct.count(t), stg);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&ctl.acc_empty[acc.slot]), 0));
@@ -510,15 +482,16 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
 
 template <bool SWIGLU, bool QOUT>
 cudaError_t launch_variant(unsigned grid, const CUtensorMap& ma, const CUtensorMap& mb,
-                           const CUtensorMap& mb1, const CUtensorMap& ms, const CUtensorMap& mc,
-                           const Params& p, cudaStream_t st) {
+                           const CUtensorMap& mb1, const CUtensorMap& ms, const CUtensorMap& ms1,
+                           const CUtensorMap& mr, const CUtensorMap& mc, const Params& p,
+                           cudaStream_t st) {
   static int done[64] = {0};
   static std::mutex mu;
   const cudaError_t e =
       allow_smem(grouped_gemm_mxfp4_pair_kernel<SWIGLU, QOUT>, kSmemBytes, done, mu);
   if (e != cudaSuccess) return e;
   return launch_pdl(kPdlGemm, grouped_gemm_mxfp4_pair_kernel<SWIGLU, QOUT>, dim3(grid),
-                    dim3(kThreads), kSmemBytes, st, ma, mb, mb1, ms, mc, p);
+                    dim3(kThreads), kSmemBytes, st, ma, mb, mb1, ms, ms1, mr, mc, p);
 }
 
 }  // namespace
@@ -527,30 +500,28 @@ cudaError_t launch_variant(unsigned grid, const CUtensorMap& ma, const CUtensorM
 cudaError_t launch_grouped_gemm_mxfp4_pair(const MxGemmArgs& a, cudaStream_t st) {
   using namespace mx;
   Params p = make_params(a);
-  const int chunks = cdiv(p.b_rows, 64);
-  p.n_tiles = cdiv(chunks, kTileChunks);
-  p.tile_chunks = chunks / p.n_tiles;
-  p.tile_extra = chunks % p.n_tiles;
   const uint64_t cb = static_cast<uint64_t>(mx_code_bytes(a.K));
-  const uint64_t nkb = cdiv(mx_padded_k(a.K), kMxKBlock);
   const uint64_t wrows = static_cast<uint64_t>(a.G) * p.b_rows;
-  CUtensorMap ma, mb, mb1, ms, mc;
+  const uint64_t atoms = static_cast<uint64_t>(mx_weight_scale_atoms(a.G, a.N, a.K, a.swiglu));
+  CUtensorMap ma, mb, mb1, ms, ms1, mr, mc;
   if (!make_code_map(&ma, a.rows, static_cast<uint64_t>(a.M), cb, p.a_row_bytes, MM) ||
-      !make_code_map(&mb, a.weight, wrows, cb, cb, 32 * p.tile_chunks) ||
-      !make_code_map(&mb1, a.weight, wrows, cb, cb, 32 * (p.tile_chunks + 1)) ||
-      !make_scale_map(&ms, p.b_scales, static_cast<uint64_t>(a.G) * p.b_chunks, nkb))
+      !make_code_map(&mb, a.weight, wrows, cb, cb, 32 * p.ct.chunks) ||
+      !make_code_map(&mb1, a.weight, wrows, cb, cb, 32 * (p.ct.chunks + 1)) ||
+      !make_scale_map(&ms, p.b_scales, atoms, p.ct.chunks) ||
+      !make_scale_map(&ms1, p.b_scales, atoms, p.ct.chunks + 1) ||
+      !make_raw_map(&mr, a.rows, static_cast<uint64_t>(a.M), p.a_row_bytes, MM))
     return cudaErrorInvalidValue;
   if (a.quantized_out)
     mc = ma;  // not used
   else if (!make_out_map(&mc, a.out, static_cast<uint64_t>(a.M), static_cast<uint64_t>(a.N)))
     return cudaErrorInvalidValue;
   const int sms = num_sms_for_current_device();
-  const int64_t max_tiles = (cdiv64(a.M, 2 * MM) + a.G) * p.n_tiles;
+  const int64_t max_tiles = (cdiv64(a.M, 2 * MM) + a.G) * p.ct.tiles;
   int pairs = static_cast<int>(max_tiles < sms / 2 ? max_tiles : sms / 2);
   if (pairs < 1) pairs = 1;
-  if (!a.swiglu) return launch_variant<false, false>(2 * pairs, ma, mb, mb1, ms, mc, p, st);
-  if (a.quantized_out) return launch_variant<true, true>(2 * pairs, ma, mb, mb1, ms, mc, p, st);
-  return launch_variant<true, false>(2 * pairs, ma, mb, mb1, ms, mc, p, st);
+  if (!a.swiglu) return launch_variant<false, false>(2 * pairs, ma, mb, mb1, ms, ms1, mr, mc, p, st);
+  if (a.quantized_out) return launch_variant<true, true>(2 * pairs, ma, mb, mb1, ms, ms1, mr, mc, p, st);
+  return launch_variant<true, false>(2 * pairs, ma, mb, mb1, ms, ms1, mr, mc, p, st);
 }
 
 }  // namespace hmoe

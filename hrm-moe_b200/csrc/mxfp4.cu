@@ -140,17 +140,24 @@ pack_weight_kernel(const uint8_t* __restrict__ codes, int64_t code_stride,
       v = *reinterpret_cast<const uint4*>(codes + (g * src_rows + src) * code_stride + c * 16);
     reinterpret_cast<uint4*>(out_codes)[i] = v;
   }
-  const int nb = cdiv(np_rows, 128), kb = cdiv(mx_padded_k(K), kMxKBlock);
-  const int64_t nscale = static_cast<int64_t>(G) * nb * kb * 1024;
+  const MxColTiles ct = mx_col_tiles(np_rows);
+  const int nkb = mx_num_kblocks(K);
+  const int atoms = cdiv(np_rows, 64) * nkb;  // of a group
+  const int64_t nscale = static_cast<int64_t>(G) * atoms * 512;
   for (int64_t i = first; i < nscale; i += step) {
     const int byte = static_cast<int>(i & 511);
-    const int64_t atom = i >> 9;
-    const int j = static_cast<int>(atom & 1);
-    const int64_t chunk = atom >> 1;
-    const int k0 = static_cast<int>(chunk % kb) * 8 + j * 4 + (byte & 3);
-    const int64_t gn = chunk / kb;
-    const int64_t g = gn / nb;
-    const int np = static_cast<int>(gn - g * nb) * 128 + ((byte >> 2) & 3) * 32 + (byte >> 4);
+    const int64_t g = (i >> 9) / atoms;
+    const int r = static_cast<int>((i >> 9) - g * atoms);
+    // tile, k-block and atom of the tile's atoms of that k-block
+    const int split = ct.extra * (ct.chunks + 1) * nkb;  // atoms of the longer tiles
+    const int t = r < split ? r / ((ct.chunks + 1) * nkb) : ct.extra + (r - split) / (ct.chunks * nkb);
+    const int nc = ct.count(t);
+    const int rt = r - ct.first(t) * nkb;
+    const int kb = rt / nc;
+    const int col = (rt - kb * nc) * 4 + ((byte >> 2) & 3);  // TMEM column of the tile
+    const int j = col / (2 * nc);                             // which 128 elements
+    const int np = ct.first(t) * 64 + (col - j * 2 * nc) * 32 + (byte >> 4);
+    const int k0 = kb * 8 + j * 4 + (byte & 3);
     uint8_t v = 0;
     if (np < np_rows && k0 < ns) {
       const int src = packed_source_row(np, N, swiglu);

@@ -10,10 +10,12 @@
 // Packed weights: the codes [G, N', K' / 2] (for gate_up weights N' =
 // 2 * ceil(I / 32) * 32 with 32 gate rows, then the 32 up rows of the same
 // features, and so on, so that a column tile holds matching gate and up
-// columns), then, 1024-byte aligned, the scales as the tensor core's
-// scale-factor atoms: [G][ceil(N' / 128)][ceil(K' / 256)][2][512], byte
-// (n % 32) * 16 + (n % 128) / 32 * 4 + s of an atom being the scale of row n,
-// block s of the atom's 128 elements.
+// columns), then, 1024-byte aligned, the scales in the order of the GEMMs'
+// column tiles.  A tile is a run of up to three 64-row chunks (the chunks of a
+// group shared out evenly); its scales of a 256-element k-block are 4 TMEM
+// columns a chunk: the columns of the first 128 elements (32 rows each, a
+// 32-bit word of 4 scales per row), then those of the second.  Four columns
+// are an atom of 512 bytes, 16 bytes for each of 32 lanes.
 #pragma once
 
 #include "common.cuh"
@@ -34,14 +36,32 @@ __host__ __device__ inline int mx_row_bytes(int K) {
 __host__ __device__ inline int mx_weight_rows(int N, int swiglu) {
   return swiglu ? 2 * mx_padded_k(N) : N;
 }
+// Column tiles of a group: `tiles` runs of 64-row chunks, the first `extra`
+// of them one longer than `chunks`.
+constexpr int kMxTileChunks = 3;
+struct MxColTiles {
+  int tiles, chunks, extra;
+  __host__ __device__ int first(int t) const { return t * chunks + (t < extra ? t : extra); }
+  __host__ __device__ int count(int t) const { return chunks + (t < extra ? 1 : 0); }
+};
+__host__ __device__ inline MxColTiles mx_col_tiles(int rows) {
+  const int chunks = cdiv(rows, 64);
+  MxColTiles t;
+  t.tiles = cdiv(chunks, kMxTileChunks);
+  t.chunks = chunks / t.tiles;
+  t.extra = chunks % t.tiles;
+  return t;
+}
+__host__ __device__ inline int mx_num_kblocks(int K) { return cdiv(mx_padded_k(K), kMxKBlock); }
 inline int64_t mx_weight_scale_offset(int G, int N, int K, int swiglu) {
   const int64_t codes = static_cast<int64_t>(G) * mx_weight_rows(N, swiglu) * mx_code_bytes(K);
   return (codes + 1023) / 1024 * 1024;
 }
+inline int64_t mx_weight_scale_atoms(int G, int N, int K, int swiglu) {
+  return static_cast<int64_t>(G) * cdiv(mx_weight_rows(N, swiglu), 64) * mx_num_kblocks(K);
+}
 inline int64_t mx_weight_bytes(int G, int N, int K, int swiglu) {
-  return mx_weight_scale_offset(G, N, K, swiglu) +
-         static_cast<int64_t>(G) * cdiv(mx_weight_rows(N, swiglu), 128) *
-             cdiv(mx_padded_k(K), kMxKBlock) * 1024;
+  return mx_weight_scale_offset(G, N, K, swiglu) + mx_weight_scale_atoms(G, N, K, swiglu) * 512;
 }
 
 // Scale byte of a block whose largest magnitude has the fp32 bits `amax`

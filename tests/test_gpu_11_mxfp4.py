@@ -207,6 +207,30 @@ def test_cta_pair_and_single_cta_kernels_agree(tmp_path):
         assert torch.equal(outs["pair"][key], outs["single"][key]), key
 
 
+@pytest.mark.parametrize("M,N,K,G", [(30000, 512, 1536, 64), (20000, 320, 1800, 4),
+                                     (4000, 512, 1536, 64), (3000, 200, 448, 100)])
+def test_products_repeat_bit_for_bit(M, N, K, G):
+    """Every run of a product gives the same bits, with cold and with warm caches
+    (a race between its copies, MMAs and epilogue would show as a difference)."""
+    ops = get_ops()
+    x = _rand((M, K), 1, dtype=torch.float32)
+    x *= torch.exp2((torch.arange(M, device="cuda") % 5).float())[:, None]  # scales by row
+    x = ops.quantize_mxfp4(x.to(torch.bfloat16))
+    w, wg = _rand((G, N, K), 2, 0.02), _rand((G, 2 * N, K), 3, 0.02)
+    pw, pg = ops.pack_mxfp4_weight(w), ops.pack_mxfp4_weight(wg, swiglu=True)
+    tpe = torch.from_numpy(ragged_counts(M, G, seed=M)).cuda()
+    calls = [lambda: ops.grouped_linear_mxfp4(x, pw, tpe),
+             lambda: ops.grouped_swiglu_mxfp4(x, pg, tpe),
+             lambda: ops.grouped_swiglu_mxfp4(x, pg, tpe, quantized=True).data]
+    want = [f() for f in calls]
+    flush = torch.empty(200 << 20, dtype=torch.uint8, device="cuda")
+    for i in range(40):
+        if i % 2:
+            flush.fill_(i)
+        for f, r in zip(calls, want):
+            assert torch.equal(f(), r)
+
+
 def test_checkpoint_and_rows_pack_alike():
     ops = get_ops()
     w = _rand((3, 80, 104), 3, 0.02, torch.float32)
