@@ -1441,13 +1441,15 @@ MxFfnBufs carve_mx_ffn(Carve& c, const hmoe_shape& s) {
   return b;
 }
 
-// Quantise, dispatch the records, the two products, combine.
+// Quantise (clearing clear_err where it is given), dispatch the records, the
+// two products, combine.
 int run_mx_experts(const hmoe_shape& s, const void* x, const int32_t* idx, const void* w,
                    int w_is_f32, const void* w_gate_up, const void* w_down, const void* final_in,
                    void* out, int32_t* counts_out, int32_t* sort_idx, const MxExpertBufs& b,
-                   cudaStream_t st) {
+                   int* clear_err, cudaStream_t st) {
   const int64_t A = s.tokens * s.top_k;
-  HMOE_CUDA(launch_mx_quantize(x, s.tokens, s.hidden, s.hidden, s.dtype, b.xq, st), "quantize_mxfp4");
+  HMOE_CUDA(launch_mx_quantize(x, s.tokens, s.hidden, s.hidden, s.dtype, b.xq, clear_err, st),
+            "quantize_mxfp4");
   hmoe_shape rec = s;  // dispatch copies records: rows of 2-byte elements
   rec.hidden = mx_row_bytes(s.hidden) / 2;
   int rc = run_dispatch(rec, idx, w, w_is_f32, b.xq, b.d, b.pos, sort_idx, nullptr, nullptr, b.xs, st);
@@ -1481,7 +1483,8 @@ int hmoe_mxfp4_quantize(const void* x, int64_t rows, int32_t K, int64_t x_stride
     return fail(HMOE_EINVAL, "x, its rows and out must be 16-byte aligned");
   DeviceScope scope;
   if ((rc = select_device(x))) return rc;
-  HMOE_CUDA(launch_mx_quantize(x, rows, K, x_stride, dtype, out, static_cast<cudaStream_t>(stream)),
+  HMOE_CUDA(launch_mx_quantize(x, rows, K, x_stride, dtype, out, nullptr,
+                               static_cast<cudaStream_t>(stream)),
             "quantize_mxfp4");
   return HMOE_OK;
 }
@@ -1567,9 +1570,8 @@ int hmoe_experts_forward_mxfp4(const hmoe_shape* shape, const void* hidden,
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   Carve c{static_cast<char*>(workspace)};
   MxExpertBufs b = carve_mx_experts(c, s);
-  HMOE_CUDA(cudaMemsetAsync(b.d.err, 0, sizeof(int), st), "reset error word");
   return run_mx_experts(s, hidden, topk_idx, topk_weight, 0, w_gate_up, w_down, final_in, y, counts,
-                        sort_idx, b, st);
+                        sort_idx, b, b.d.err, st);
 }
 
 size_t hmoe_ffn_mxfp4_workspace_bytes(const hmoe_shape* shape) {
@@ -1602,7 +1604,7 @@ int hmoe_ffn_forward_mxfp4(const hmoe_shape* shape, const void* x, const void* w
                        b.router_scratch, b.x.d.err, st, true),
             "router_topk");
   return run_mx_experts(s, x, idx, b.topk_w, 1, w_gate_up, w_down, accumulate ? y : nullptr, y,
-                        counts, sort_idx, b.x, st);
+                        counts, sort_idx, b.x, nullptr, st);
 }
 
 }  // extern "C"

@@ -198,13 +198,6 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
   return g * r * u;
 }
 
-// max(|a|, |b|, c), NaN if any is.
-__device__ __forceinline__ float max3_abs(float a, float b, float c) {
-  float r;
-  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
 // 32 output columns of one row, as a warp: quantised to a record's block, or
 // rounded to bf16 and stored as a whole 32 x 32 box by TMA where all 32 rows
 // are the group's, else row by row.

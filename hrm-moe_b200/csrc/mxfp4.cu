@@ -9,103 +9,201 @@ namespace {
 
 constexpr int kQThreads = 256;
 
-// |x| of two bf16 as bits: the maximum of bf16 magnitudes orders as unsigned
-// 16-bit integers, NaN above everything.
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
-  return __vmaxu2(a, b);
+// One thread per block of 32: the maximum and the scale are the thread's own,
+// its 16 bytes of codes are one store.  The kernels are short of instruction
+// slots before they are short of bandwidth, so the work is kept in packed
+// bf16 pairs.  (Four lanes to a block, 8 elements each, took 126 instructions
+// per 8 elements and 20 us for [16384, 1536] bf16; the way back, element by
+// element, 238 and 28 us.)  A CTA takes whole rows, so that one 32-bit
+// multiply finds a block's row.
+struct RowSplit {
+  int rows_per_cta, blocks;  // blocks of a row
+  uint32_t magic;            // ceil(2^32 / blocks)
+};
+RowSplit row_split(int blocks) {
+  RowSplit r;
+  r.blocks = blocks;
+  r.rows_per_cta = blocks < kQThreads ? kQThreads / blocks : 1;
+  r.magic = static_cast<uint32_t>(((1ull << 32) + blocks - 1) / blocks);
+  return r;
+}
+// Row of block i of a CTA.  Exact: with several rows to a CTA, i * blocks <
+// 2 * kQThreads^2 < 2^32; with one row it is 0, and with one block to a row
+// (whose magic number does not fit) it is i.
+__device__ __forceinline__ int block_row(const RowSplit& sp, int i) {
+  if (sp.rows_per_cta == 1) return 0;
+  return sp.blocks == 1 ? i : static_cast<int>(__umulhi(static_cast<uint32_t>(i), sp.magic));
 }
 
-// One thread per 8 elements (a 16-byte load of bf16, two of fp32), four lanes
-// per block of 32: the block's maximum is two shuffles, a lane's 8 codes are
-// one 32-bit word, and lane 0 of the four stores the scale byte.  Elements
-// past K are zeros; the lanes past the last block fill the record's padding.
-template <bool BF16>
+// Loads of what the kernel before may have written: volatile, and nothing in
+// these kernels is const __restrict__ or __ldg, so that the compiler moves no
+// load above griddepcontrol.wait.
+__device__ __forceinline__ void ld_32bytes(const void* p, uint32_t* w) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]),
+        "=r"(w[7])
+      : "l"(p)
+      : "memory");
+}
+__device__ __forceinline__ uint4 ld_16bytes(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t max_abs_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("{\n\t.reg .b32 x;\n\tabs.bf16x2 x, %2;\n\tmax.NaN.bf16x2 %0, %1, x;\n\t}"
+      : "=r"(r)
+      : "r"(a), "r"(b));
+  return r;
+}
+
+// WIDE: whole blocks, rows 32-byte aligned (two or four 32-byte loads a block);
+// else 16-byte loads, each of which may lie behind K (a multiple of 8).
+template <bool BF16, bool WIDE>
 __global__ void __launch_bounds__(kQThreads)
-quantize_kernel(const void* __restrict__ x, int64_t rows, int K, int64_t x_stride,
-                uint8_t* __restrict__ out) {
+quantize_kernel(const void* x, int64_t rows, int K, int64_t x_stride, RowSplit sp, uint8_t* out,
+                int* err) {
   grid_dependency_wait();  // launched early (launch_pdl)
   grid_launch_dependents();
-  const int row_bytes = mx_row_bytes(K);
-  const int cb = mx_code_bytes(K), ns = mx_num_scales(K);
-  const int lanes_per_row = 4 * ns;  // 8 elements each
-  const int64_t total = rows * lanes_per_row;
-  // every lane of a warp runs the same trip count (the shuffles see all lanes)
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * kQThreads + (threadIdx.x & ~31);
-       base < total; base += static_cast<int64_t>(gridDim.x) * kQThreads) {
-    const int64_t i = base + (threadIdx.x & 31);
-    const bool live = i < total;
-    const int64_t r = live ? i / lanes_per_row : 0;
-    const int c = live ? static_cast<int>(i - r * lanes_per_row) : 0;  // 8-element chunk of the row
-    float v[8];
-    uint32_t amax = 0;
-    if (live && c * 8 < K) {  // K is a multiple of 8
-      if (BF16) {
-        const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) +
-                                                        r * x_stride + c * 8);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  if (err && blockIdx.x == 0 && threadIdx.x == 0) *err = 0;
+  const int row_bytes = mx_row_bytes(K), cb = mx_code_bytes(K);
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * sp.rows_per_cta;
+  const int nrows = static_cast<int>(rows - row0 < sp.rows_per_cta ? rows - row0 : sp.rows_per_cta);
+  const int total = nrows * sp.blocks;
+  for (int i = threadIdx.x; i < total; i += kQThreads) {
+    const int r = block_row(sp, i);
+    const int b = i - r * sp.blocks;
+    constexpr int kWords = BF16 ? 16 : 32;
+    constexpr int ES = BF16 ? 2 : 4;
+    uint32_t w[kWords];
+    const uint8_t* src =
+        static_cast<const uint8_t*>(x) + ((row0 + r) * x_stride + b * kMxBlock) * ES;
+    if (WIDE) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { v[2 * j] = bf16_lo(w[j]); v[2 * j + 1] = bf16_hi(w[j]); }
-        const uint32_t m = max_u16x2(max_u16x2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu),
-                                     max_u16x2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
-        amax = max(m >> 16, m & 0xffffu) << 16;
-      } else {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) +
-                                                          r * x_stride + c * 8);
-        const float4 a = p[0], b = p[1];
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
-      }
+      for (int h = 0; h < kWords / 8; ++h) ld_32bytes(src + 32 * h, w + 8 * h);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+      for (int h = 0; h < kWords / 4; ++h) {
+        const uint4 q = b * kMxBlock + h * (16 / ES) < K
+                            ? ld_16bytes(src + 16 * h)
+                            : make_uint4(0, 0, 0, 0);
+        w[4 * h] = q.x; w[4 * h + 1] = q.y; w[4 * h + 2] = q.z; w[4 * h + 3] = q.w;
+      }
     }
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    if (!live) continue;  // whole groups of four lanes: total is a multiple of 4
+    uint32_t amax;
+    if (BF16) {
+      uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+      for (int j = 1; j < 16; ++j) m = max_abs_bf16x2(m, w[j]);
+      amax = max_abs_bf16x2(m, m >> 16) << 16;
+    } else {
+      float m = fabsf(__uint_as_float(w[0]));
+#pragma unroll
+      for (int j = 1; j < 31; j += 2)
+        m = max3_abs(__uint_as_float(w[j]), __uint_as_float(w[j + 1]), m);
+      amax = __float_as_uint(max3_abs(__uint_as_float(w[31]), m, m));
+    }
     const uint32_t s = mx_scale_code(amax);
     const float inv = mx_inv_scale(s);
-    uint8_t* row = out + r * row_bytes;
-    reinterpret_cast<uint32_t*>(row)[c] =
-        mx_cvt8(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv, v[4] * inv, v[5] * inv, v[6] * inv,
-                v[7] * inv);
-    if ((c & 3) == 0) {
-      row[cb + (c >> 2)] = static_cast<uint8_t>(s);
-      if ((c >> 2) == ns - 1)
-        for (int b = cb + ns; b < row_bytes; ++b) row[b] = 0;
+    uint32_t q[4];
+    if (BF16) {
+      // x / s in bf16: exact (a power of two), or so small that its code is 0
+      const uint32_t inv2 = cvt_bf16x2(inv, inv);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) w[j] = mul_bf16x2(w[j], inv2);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        q[j] = mx_cvt8(bf16_lo(w[4 * j]), bf16_hi(w[4 * j]), bf16_lo(w[4 * j + 1]),
+                       bf16_hi(w[4 * j + 1]), bf16_lo(w[4 * j + 2]), bf16_hi(w[4 * j + 2]),
+                       bf16_lo(w[4 * j + 3]), bf16_hi(w[4 * j + 3]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(w[(8 * j + e) % kWords]) * inv;
+        q[j] = mx_cvt8(f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]);
+      }
     }
+    uint8_t* o = out + (row0 + r) * row_bytes;
+    reinterpret_cast<uint4*>(o)[b] = make_uint4(q[0], q[1], q[2], q[3]);
+    o[cb + b] = static_cast<uint8_t>(s);
+    if (b == sp.blocks - 1)
+      for (int z = cb + sp.blocks; z < row_bytes; ++z) o[z] = 0;
   }
 }
 
-template <bool BF16>
+// Four codes (the low 16 bits of w) -> their values as two bf16 pairs: the
+// bytes of the eight magnitudes are looked up by byte permutes, the sign bits
+// likewise.
+__device__ __forceinline__ void values4(uint32_t w, uint32_t& v01, uint32_t& v23) {
+  const uint32_t sel = w & 0x7777u;
+  // 0, .5, 1, 1.5, 2, 3, 4, 6: 0x0000 3f00 3f80 3fc0 4000 4040 4080 40c0
+  const uint32_t lo = __byte_perm(0xc0800000u, 0xc0804000u, sel);
+  const uint32_t hi = __byte_perm(0x3f3f3f00u, 0x40404040u, sel) |
+                      __byte_perm(0x00008000u, 0u, (w >> 3) & 0x1111u);
+  v01 = __byte_perm(lo, hi, 0x5140u);
+  v23 = __byte_perm(lo, hi, 0x7362u);
+}
+
+// WIDE: whole blocks, 32-byte aligned output rows.
+template <bool BF16, bool WIDE>
 __global__ void __launch_bounds__(kQThreads)
-dequantize_kernel(const uint8_t* __restrict__ rows_in, int64_t rows, int K,
-                  void* __restrict__ out) {
+dequantize_kernel(const uint8_t* rows_in, int64_t rows, int K, RowSplit sp, void* out) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int row_bytes = mx_row_bytes(K), cb = mx_code_bytes(K);
-  const int chunks = K / 8;
-  const int64_t total = rows * chunks;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kQThreads + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * kQThreads) {
-    const int64_t r = i / chunks;
-    const int c = static_cast<int>(i - r * chunks);
-    const uint8_t* row = rows_in + r * row_bytes;
-    const uint32_t w = reinterpret_cast<const uint32_t*>(row)[c];
-    const uint32_t s = row[cb + (c >> 2)];
-    float v[8];
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * sp.rows_per_cta;
+  const int nrows = static_cast<int>(rows - row0 < sp.rows_per_cta ? rows - row0 : sp.rows_per_cta);
+  const int total = nrows * sp.blocks;
+  for (int i = threadIdx.x; i < total; i += kQThreads) {
+    const int r = block_row(sp, i);
+    const int b = i - r * sp.blocks;
+    const uint8_t* row = rows_in + (row0 + r) * row_bytes;
+    const uint4 c = ld_16bytes(row + 16 * b);
+    const uint32_t s = row[cb + b];
+    // the scale in bf16: 2^-127 is a subnormal, 255 is NaN
+    const uint32_t sb = s == 255u ? 0x7fc0u : s == 0u ? 0x0040u : s << 7;
+    const uint32_t s2 = sb | sb << 16;
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    uint32_t v[16];  // exact: two significant bits, and 2^-128 is a bf16 subnormal
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = mx_value((w >> (4 * j)) & 15u, s);
-    if (BF16) {
-      // exact: two significant bits, and 2^-128 is a bf16 subnormal
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + r * K + c * 8) =
-          make_uint4(cvt_bf16x2(v[0], v[1]), cvt_bf16x2(v[2], v[3]), cvt_bf16x2(v[4], v[5]),
-                     cvt_bf16x2(v[6], v[7]));
-    } else {
-      float4* p = reinterpret_cast<float4*>(static_cast<float*>(out) + r * K + c * 8);
-      p[0] = make_float4(v[0], v[1], v[2], v[3]);
-      p[1] = make_float4(v[4], v[5], v[6], v[7]);
+    for (int j = 0; j < 4; ++j) {
+      values4(w[j], v[4 * j], v[4 * j + 1]);
+      values4(w[j] >> 16, v[4 * j + 2], v[4 * j + 3]);
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = mul_bf16x2(v[j], s2);
+    constexpr int ES = BF16 ? 2 : 4;
+    uint8_t* dst = static_cast<uint8_t*>(out) + ((row0 + r) * K + b * kMxBlock) * ES;
+    constexpr int kParts = BF16 ? 4 : 8;  // 16-byte stores
+#pragma unroll
+    for (int h = 0; h < kParts; h += 2) {
+      uint4 q[2];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        if (BF16)
+          q[g] = make_uint4(v[4 * ((h + g) % 4)], v[4 * ((h + g) % 4) + 1], v[4 * ((h + g) % 4) + 2],
+                            v[4 * ((h + g) % 4) + 3]);
+        else
+          q[g] = make_uint4(v[2 * (h + g)] << 16, v[2 * (h + g)] & 0xffff0000u,
+                            v[2 * (h + g) + 1] << 16, v[2 * (h + g) + 1] & 0xffff0000u);
+      }
+      if (WIDE) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 16 * h),
+                     "r"(q[0].x), "r"(q[0].y), "r"(q[0].z), "r"(q[0].w), "r"(q[1].x), "r"(q[1].y),
+                     "r"(q[1].z), "r"(q[1].w)
+                     : "memory");
+      } else {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          if (b * kMxBlock + (h + g) * (16 / ES) < K)
+            *reinterpret_cast<uint4*>(dst + 16 * (h + g)) = q[g];
+      }
     }
   }
 }
@@ -174,9 +272,9 @@ pack_weight_kernel(const uint8_t* __restrict__ codes, int64_t code_stride,
 // the k rows of a column block are loaded before they are summed, in slot
 // order.
 __global__ void __launch_bounds__(kQThreads, 4)
-combine_f32_kernel(const uint4* __restrict__ rows, const int32_t* __restrict__ pos,
-                   const void* __restrict__ topk_w, int topk_w_is_f32, int64_t T, int row_chunks,
-                   int k, int warps_per_token, const uint4* final_in, uint4* out) {
+combine_f32_kernel(const uint4* rows, const int32_t* pos, const void* topk_w, int topk_w_is_f32,
+                   int64_t T, int row_chunks, int k, int warps_per_token, const uint4* final_in,
+                   uint4* out) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int lane = threadIdx.x & 31;
@@ -211,7 +309,7 @@ combine_f32_kernel(const uint4* __restrict__ rows, const int32_t* __restrict__ p
       for (int b = 0; b < kBatch; ++b) {
         const int pj = j0 + b < k ? __shfl_sync(0xffffffffu, p, (j0 + b) & 31) : -1;
         ws[b] = __shfl_sync(0xffffffffu, w, (j0 + b) & 31);
-        v[b] = live && pj >= 0 ? __ldg(rows + static_cast<int64_t>(pj) * row_chunks + c)
+        v[b] = live && pj >= 0 ? ld_16bytes(rows + static_cast<int64_t>(pj) * row_chunks + c)
                                : make_uint4(0, 0, 0, 0);
         if (pj < 0) ws[b] = 0.0f;  // a dropped assignment adds nothing, whatever its weight
       }
@@ -240,25 +338,32 @@ unsigned stream_blocks(int64_t threads) {
 }  // namespace
 
 cudaError_t launch_mx_quantize(const void* x, int64_t rows, int K, int64_t x_stride, int dtype,
-                               void* out, cudaStream_t st) {
+                               void* out, int* clear_err, cudaStream_t st) {
   if (rows == 0) return cudaSuccess;
-  const dim3 grid(stream_blocks(rows * 4 * mx_num_scales(K)));
-  if (dtype == kDtypeBF16)
-    return launch_pdl(kPdlDispatch, quantize_kernel<true>, grid, dim3(kQThreads), 0, st, x, rows, K,
-                      x_stride, static_cast<uint8_t*>(out));
-  return launch_pdl(kPdlDispatch, quantize_kernel<false>, grid, dim3(kQThreads), 0, st, x, rows, K,
-                    x_stride, static_cast<uint8_t*>(out));
+  const RowSplit sp = row_split(mx_num_scales(K));
+  const int64_t ctas = cdiv64(rows, sp.rows_per_cta);
+  if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
+  const bool bf16 = dtype == kDtypeBF16;
+  const bool wide = K % kMxBlock == 0 && reinterpret_cast<uintptr_t>(x) % 32 == 0 &&
+                    x_stride * (bf16 ? 2 : 4) % 32 == 0;
+  const auto kernel = bf16 ? (wide ? quantize_kernel<true, true> : quantize_kernel<true, false>)
+                           : (wide ? quantize_kernel<false, true> : quantize_kernel<false, false>);
+  return launch_pdl(kPdlDispatch, kernel, dim3(static_cast<unsigned>(ctas)), dim3(kQThreads), 0, st,
+                    x, rows, K, x_stride, sp, static_cast<uint8_t*>(out), clear_err);
 }
 
 cudaError_t launch_mx_dequantize(const void* rows_in, int64_t rows, int K, int dtype, void* out,
                                  cudaStream_t st) {
   if (rows == 0) return cudaSuccess;
-  const dim3 grid(stream_blocks(rows * (K / 8)));
-  if (dtype == kDtypeBF16)
-    return launch_pdl(kPdlDispatch, dequantize_kernel<true>, grid, dim3(kQThreads), 0, st,
-                      static_cast<const uint8_t*>(rows_in), rows, K, out);
-  return launch_pdl(kPdlDispatch, dequantize_kernel<false>, grid, dim3(kQThreads), 0, st,
-                    static_cast<const uint8_t*>(rows_in), rows, K, out);
+  const RowSplit sp = row_split(mx_num_scales(K));
+  const int64_t ctas = cdiv64(rows, sp.rows_per_cta);
+  if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
+  const bool bf16 = dtype == kDtypeBF16;
+  const bool wide = K % kMxBlock == 0 && reinterpret_cast<uintptr_t>(out) % 32 == 0;
+  const auto kernel = bf16 ? (wide ? dequantize_kernel<true, true> : dequantize_kernel<true, false>)
+                           : (wide ? dequantize_kernel<false, true> : dequantize_kernel<false, false>);
+  return launch_pdl(kPdlDispatch, kernel, dim3(static_cast<unsigned>(ctas)), dim3(kQThreads), 0, st,
+                    static_cast<const uint8_t*>(rows_in), rows, K, sp, out);
 }
 
 cudaError_t launch_mx_pack_weight(const void* codes, int64_t code_stride, const void* scales,

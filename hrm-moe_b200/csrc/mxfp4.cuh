@@ -94,15 +94,11 @@ __device__ __forceinline__ uint32_t mx_cvt8(float v0, float v1, float v2, float 
   return r;
 }
 
-// The value of a 4-bit code, times 2^(scale - 127) (exact).
-__device__ __forceinline__ float mx_value(uint32_t code, uint32_t scale) {
-  const uint32_t m = code & 7u;
-  // e2m1 magnitude: 0, 0.5, 1, 1.5, 2, 3, 4, 6
-  const float mag = m < 2u ? 0.5f * m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
-  if (scale == 255u) return __uint_as_float(0x7fc00000u);
-  // 2^(scale - 127) in two factors: 2^-127 is a subnormal
-  const float s = scale >= 1u ? __uint_as_float(scale << 23) : __uint_as_float(0x00400000u);
-  return (code & 8u ? -mag : mag) * s;
+// max(|a|, |b|, |c|), NaN if any is.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 }  // namespace hmoe

@@ -415,10 +415,24 @@ def ffn_forward(x: torch.Tensor, w_router: torch.Tensor, w_gate_up: torch.Tensor
 
 
 # ------------------------------------------------------------------- MXFP4 --
-def _inference_only(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no backward (MXFP4 is for inference): call it under "
-                           "torch.no_grad() or torch.inference_mode()")
+# These calls are short at decode sizes, so the host path is kept lean: plain
+# integers for pointers, the raw stream handle, no repeated validation of
+# objects made here.
+def _refuse_grad(what: str) -> None:
+    raise RuntimeError(f"{what} has no backward (MXFP4 is for inference): call it under "
+                       "torch.no_grad() or torch.inference_mode()")
+
+
+def _raw_stream(dev: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _mxfp4_row_bytes(k: int) -> int:
+    """hmoe_mxfp4_row_bytes: codes, scales filled up to 8 bytes, the record to 16."""
+    if k <= 0 or k % 8 or k > 1 << 24:
+        raise ValueError(f"K must be a positive multiple of 8 (at most 2^24), got {k}")
+    blocks = (k + 31) // 32
+    return (16 * blocks + (blocks + 7) // 8 * 8 + 15) // 16 * 16
 
 
 class Mxfp4Rows:
@@ -430,10 +444,10 @@ class Mxfp4Rows:
     being K filled up to whole blocks with zeros.
     """
 
+    __slots__ = ("data", "k")
+
     def __init__(self, data: torch.Tensor, k: int):
-        row_bytes = _lib.load().hmoe_mxfp4_row_bytes(int(k))
-        if row_bytes == 0:
-            raise ValueError(_lib.last_error())
+        row_bytes = _mxfp4_row_bytes(int(k))
         if data.dtype != torch.uint8:
             raise TypeError(f"MXFP4 records are uint8, got {data.dtype}")
         if data.dim() < 1 or data.shape[-1] != row_bytes or not data.is_contiguous():
@@ -441,6 +455,12 @@ class Mxfp4Rows:
                              f"{tuple(data.shape)}")
         self.data = data
         self.k = int(k)
+
+    @classmethod
+    def _of(cls, data: torch.Tensor, k: int) -> "Mxfp4Rows":
+        rows = cls.__new__(cls)
+        rows.data, rows.k = data, k
+        return rows
 
     @property
     def shape(self) -> torch.Size:
@@ -452,20 +472,21 @@ class Mxfp4Rows:
 
     @property
     def codes(self) -> torch.Tensor:
-        return self.data[..., : -(-self.k // 32) * 16]
+        return self.data[..., : (self.k + 31) // 32 * 16]
 
     @property
     def scales(self) -> torch.Tensor:
-        blocks = -(-self.k // 32)
+        blocks = (self.k + 31) // 32
         return self.data[..., 16 * blocks: 17 * blocks]
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values the rows stand for (bf16 and fp32 both hold them exactly)."""
         code = dtype_code(dtype)
-        dev = _require_cuda(self.data)
-        out = torch.empty(self.shape, dtype=dtype, device=dev)
-        _lib.check(_lib.load().hmoe_mxfp4_dequantize(
-            _ptr(self.data), out.numel() // self.k, self.k, code, _ptr(out), _stream(dev)))
+        data, k = self.data, self.k
+        dev = _require_cuda(data)
+        out = torch.empty((*data.shape[:-1], k), dtype=dtype, device=dev)
+        _lib.check(_lib.load().hmoe_mxfp4_dequantize(data.data_ptr(), out.numel() // k, k, code,
+                                                     out.data_ptr(), _raw_stream(dev)))
         return out
 
 
@@ -476,27 +497,28 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Rows:
     even and saturate at 6 scales; a block with an infinity or a NaN becomes
     NaN.
     """
-    _inference_only("quantize_mxfp4", x)
+    if x.requires_grad and torch.is_grad_enabled():
+        _refuse_grad("quantize_mxfp4")
     code = dtype_code(x.dtype)
     dev = _require_cuda(x)
-    if x.dim() < 1:
+    shape = x.shape
+    if not shape:
         raise ValueError("quantize_mxfp4 takes rows [..., K]")
-    k = x.shape[-1]
-    lib = _lib.load()
-    row_bytes = lib.hmoe_mxfp4_row_bytes(k)
-    if row_bytes == 0:
-        raise ValueError(_lib.last_error())
-    es = x.element_size()
-    if not (x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= k
-            and x.stride(0) * es % 16 == 0 and x.data_ptr() % 16 == 0):
+    k = shape[-1]
+    row_bytes = _mxfp4_row_bytes(k)
+    stride, align = k, 8 if code == _lib.DTYPE_BF16 else 4
+    if len(shape) == 2 and x.stride(1) == 1 and x.stride(0) >= k and x.stride(0) % align == 0:
+        stride = x.stride(0)
+    else:
         x = x.contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone()
-    data = torch.empty((*x.shape[:-1], row_bytes), dtype=torch.uint8, device=dev)
-    rows = data.numel() // row_bytes
-    _lib.check(lib.hmoe_mxfp4_quantize(_ptr(x), rows, k, x.stride(0) if x.dim() == 2 else k, code,
-                                       _ptr(data), _stream(dev)))
-    return Mxfp4Rows(data, k)
+    ptr = x.data_ptr()
+    if ptr % 16:
+        x = x.contiguous().clone()
+        ptr, stride = x.data_ptr(), k
+    data = torch.empty((*shape[:-1], row_bytes), dtype=torch.uint8, device=dev)
+    _lib.check(_lib.load().hmoe_mxfp4_quantize(ptr, data.numel() // row_bytes, k, stride, code,
+                                               data.data_ptr(), _raw_stream(dev)))
+    return Mxfp4Rows._of(data, k)
 
 
 class Mxfp4Weight:
@@ -505,6 +527,8 @@ class Mxfp4Weight:
     [groups, n, k] for ``grouped_linear_mxfp4``; with ``swiglu`` the gate and
     up halves of [groups, 2n, k] for ``grouped_swiglu_mxfp4``.
     """
+
+    __slots__ = ("data", "groups", "n", "k", "swiglu")
 
     def __init__(self, data: torch.Tensor, groups: int, n: int, k: int, swiglu: bool):
         self.data, self.groups, self.n, self.k, self.swiglu = data, groups, n, k, swiglu
@@ -568,35 +592,36 @@ def _grouped_mxfp4(what: str, x, weight: Mxfp4Weight, tokens_per_expert: torch.T
         raise TypeError(f"{what} takes a weight from pack_mxfp4_weight, got {type(weight).__name__}")
     if weight.swiglu != swiglu:
         raise ValueError(f"{what} needs a weight packed with swiglu={swiglu}")
+    G, n, k = weight.groups, weight.n, weight.k
     if not isinstance(x, Mxfp4Rows):
-        _inference_only(what, x)
-        if x.dim() == 2 and x.shape[1] != weight.k:
-            raise ValueError(f"grouped GEMM K mismatch: input K={x.shape[1]}, weight K={weight.k}")
+        if x.requires_grad and torch.is_grad_enabled():
+            _refuse_grad(what)
+        if x.dim() == 2 and x.shape[1] != k:
+            raise ValueError(f"grouped GEMM K mismatch: input K={x.shape[1]}, weight K={k}")
         x = quantize_mxfp4(x)
-    if len(x.shape) != 2 or x.k != weight.k:
-        raise ValueError(f"grouped GEMM K mismatch: input {tuple(x.shape)}, weight K={weight.k}")
-    if tokens_per_expert.numel() != weight.groups:
-        raise ValueError(f"tokens_per_expert has {tokens_per_expert.numel()} entries, weight has "
-                         f"{weight.groups} groups")
-    dev = _require_cuda(x.data, weight.data, tokens_per_expert)
-    M = x.shape[0]
+    rows = x.data
+    if rows.dim() != 2 or x.k != k:
+        raise ValueError(f"grouped GEMM K mismatch: input {tuple(x.shape)}, weight K={k}")
     tpe = tokens_per_expert
+    if tpe.numel() != G:
+        raise ValueError(f"tokens_per_expert has {tpe.numel()} entries, weight has {G} groups")
+    dev = _require_cuda(rows, weight.data, tpe)
+    M = rows.shape[0]
     if tpe.dtype != torch.int32 or not tpe.is_contiguous():
         tpe = tpe.to(torch.int32).contiguous()
     lib = _lib.load()
     if quantized:
-        out = torch.empty((M, lib.hmoe_mxfp4_row_bytes(weight.n)), dtype=torch.uint8, device=dev)
+        out = torch.empty((M, _mxfp4_row_bytes(n)), dtype=torch.uint8, device=dev)
     else:
-        out = torch.empty((M, weight.n), dtype=torch.bfloat16, device=dev)
+        out = torch.empty((M, n), dtype=torch.bfloat16, device=dev)
+    args = (rows.data_ptr(), weight.data.data_ptr(), tpe.data_ptr(), M, n, k, G)
     if swiglu:
-        _lib.check(lib.hmoe_grouped_swiglu_mxfp4(
-            _ptr(x.data), _ptr(weight.data), _ptr(tpe), M, weight.n, weight.k, weight.groups,
-            int(quantized), _ptr(out), None, 0, _stream(dev)))
+        rc = lib.hmoe_grouped_swiglu_mxfp4(*args, int(quantized), out.data_ptr(), None, 0,
+                                           _raw_stream(dev))
     else:
-        _lib.check(lib.hmoe_grouped_linear_mxfp4(
-            _ptr(x.data), _ptr(weight.data), _ptr(tpe), M, weight.n, weight.k, weight.groups,
-            _ptr(out), None, 0, _stream(dev)))
-    return Mxfp4Rows(out, weight.n) if quantized else out
+        rc = lib.hmoe_grouped_linear_mxfp4(*args, out.data_ptr(), None, 0, _raw_stream(dev))
+    _lib.check(rc)
+    return Mxfp4Rows._of(out, n) if quantized else out
 
 
 def grouped_linear_mxfp4(x, weight: Mxfp4Weight, tokens_per_expert: torch.Tensor) -> torch.Tensor:
@@ -647,7 +672,9 @@ def experts_forward_mxfp4(hidden_states: torch.Tensor, selected_experts: torch.T
     place and returns it.  The products sum in fp32, each expert's output is
     bf16, and a token's weighted sum is fp32 rounded once.  Inference only.
     """
-    _inference_only("experts_forward_mxfp4", hidden_states, routing_weights, final_hidden_states)
+    if torch.is_grad_enabled() and (hidden_states.requires_grad or routing_weights.requires_grad or (
+            final_hidden_states is not None and final_hidden_states.requires_grad)):
+        _refuse_grad("experts_forward_mxfp4")
     T, d = hidden_states.shape
     k = selected_experts.shape[-1]
     shape = _mxfp4_shape(T, d, hidden_states.dtype, k, w_gate_up, w_down)
@@ -661,18 +688,27 @@ def experts_forward_mxfp4(hidden_states: torch.Tensor, selected_experts: torch.T
                          "place)")
     if T == 0:
         return out
-    hs = hidden_states.contiguous()
-    idx = selected_experts.reshape(T, k).to(torch.int32).contiguous()
-    rw = routing_weights.reshape(T, k).to(torch.bfloat16).contiguous()
+    hs, idx, rw = hidden_states, selected_experts, routing_weights
+    if not hs.is_contiguous():
+        hs = hs.contiguous()
+    if idx.dtype != torch.int32 or not idx.is_contiguous():
+        idx = idx.reshape(T, k).to(torch.int32).contiguous()
+    if rw.dtype != torch.bfloat16 or not rw.is_contiguous():
+        rw = rw.reshape(T, k).to(torch.bfloat16).contiguous()
+    if idx.numel() != T * k or rw.numel() != T * k:
+        raise ValueError(f"selected_experts {tuple(selected_experts.shape)} and routing_weights "
+                         f"{tuple(routing_weights.shape)} do not match {T} tokens")
     lib = _lib.load()
-    ws_bytes = lib.hmoe_experts_mxfp4_workspace_bytes(ctypes.byref(shape))
+    shape = ctypes.byref(shape)
+    ws_bytes = lib.hmoe_experts_mxfp4_workspace_bytes(shape)
     if ws_bytes == 0:
         raise ValueError(_lib.last_error())
     ws = _workspace(ws_bytes, dev)
     _lib.check(lib.hmoe_experts_forward_mxfp4(
-        ctypes.byref(shape), _ptr(hs), _ptr(idx), _ptr(rw), _ptr(w_gate_up.data),
-        _ptr(w_down.data), _ptr(final_hidden_states), _ptr(out), _ptr(counts_out),
-        _ptr(sort_idx_out), _ptr(ws), ws.numel(), _stream(dev)))
+        shape, hs.data_ptr(), idx.data_ptr(), rw.data_ptr(), w_gate_up.data.data_ptr(),
+        w_down.data.data_ptr(), None if final_hidden_states is None else out.data_ptr(),
+        out.data_ptr(), _ptr(counts_out), _ptr(sort_idx_out), ws.data_ptr(), ws.numel(),
+        _raw_stream(dev)))
     return out
 
 
@@ -683,7 +719,9 @@ def ffn_forward_mxfp4(x: torch.Tensor, w_router: torch.Tensor, w_gate_up: Mxfp4W
                       return_routing: bool = False):
     """``ffn_forward`` with MXFP4 expert weights: the bf16 router (same routing), then
     the experts as in :func:`experts_forward_mxfp4`.  Inference only."""
-    _inference_only("ffn_forward_mxfp4", x, w_router, router_bias)
+    if torch.is_grad_enabled() and (x.requires_grad or w_router.requires_grad or (
+            router_bias is not None and router_bias.requires_grad)):
+        _refuse_grad("ffn_forward_mxfp4")
     T, d = x.shape
     dt = x.dtype
     shape = _mxfp4_shape(T, d, dt, top_k, w_gate_up, w_down, norm_topk_prob)

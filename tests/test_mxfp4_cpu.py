@@ -14,7 +14,7 @@ from _helpers import package
 
 @pytest.fixture(scope="module")
 def lib():
-    package().build()
+    package()
     return importlib.import_module("hrm-moe_b200._lib")
 
 
