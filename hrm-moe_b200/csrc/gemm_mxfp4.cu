@@ -44,9 +44,12 @@ struct Ctl {
 };
 constexpr int kOffRaw = ST * kStageBytes;  // [128 rows][16 scales]
 constexpr int kOffEpi = kOffRaw + kRaw * 2048;
-constexpr int kOffCtl = kOffEpi + kEpiWarps * kEpiBox;
-constexpr size_t kSmemBytes = 1024 + kOffCtl + sizeof(Ctl);
-static_assert(kSmemBytes <= 232448, "shared memory budget of one sm_100 CTA");
+template <bool QOUT>
+constexpr int kOffCtl = kOffEpi + epi_bytes<QOUT>();
+template <bool QOUT>
+constexpr size_t kSmemBytes = 1024 + kOffCtl<QOUT> + sizeof(Ctl);
+static_assert(kSmemBytes<false> <= 232448 && kSmemBytes<true> <= 232448,
+              "shared memory budget of one sm_100 CTA");
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
                                           uint32_t bar) {
@@ -78,7 +81,7 @@ grouped_gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  Ctl& ctl = *reinterpret_cast<Ctl*>(smem + kOffCtl);
+  Ctl& ctl = *reinterpret_cast<Ctl*>(smem + kOffCtl<QOUT>);
   const uint32_t sbase = smem_u32(smem);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -285,17 +288,20 @@ grouped_gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
   } else {
     // ------------------------------------------------------------ epilogue
     const int w = warp - 4;
-    const uint32_t stg = sbase + kOffEpi + w * kEpiBox;
     Ring acc;
+    bool live = true;  // false once a wait gave up: the rest without work
+    int buf = 0;
     for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x) {
       const Tile t = decode_tile(ctl.tab, p, tile);
-      if (!wait(ctl.acc_full[acc.slot], acc.phase)) break;
+      live = live && wait(ctl.acc_full[acc.slot], acc.phase);
       tc_fence_after();
       epilogue_tile<SWIGLU, QOUT>(p, &tmC, w, tmem_base + acc.slot * kAccCols, t.row0,
-                                  min(MM, t.row_end - t.row0), t.c0, t.nc, stg);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&ctl.acc_empty[acc.slot]));
+                                  min(MM, t.row_end - t.row0), t.c0, t.nc, sbase + kOffEpi, buf, live,
+                                  [&] {
+                                    tc_fence_before();
+                                    __syncwarp();
+                                    if (lane == 0) mbar_arrive(smem_u32(&ctl.acc_empty[acc.slot]));
+                                  });
       acc.next(kAccs);
     }
     if (lane == 0) bulk_wait_group_all();
@@ -338,10 +344,10 @@ cudaError_t launch_variant(unsigned grid, const CUtensorMap& ma, const CUtensorM
   static int done[64] = {0};
   static std::mutex mu;
   const cudaError_t e =
-      allow_smem(grouped_gemm_mxfp4_kernel<SWIGLU, QOUT>, kSmemBytes, done, mu);
+      allow_smem(grouped_gemm_mxfp4_kernel<SWIGLU, QOUT>, kSmemBytes<QOUT>, done, mu);
   if (e != cudaSuccess) return e;
   return launch_pdl(kPdlGemm, grouped_gemm_mxfp4_kernel<SWIGLU, QOUT>, dim3(grid), dim3(kThreads),
-                    kSmemBytes, st, ma, mb, mr, mc, p);
+                    kSmemBytes<QOUT>, st, ma, mb, mr, mc, p);
 }
 
 }  // namespace

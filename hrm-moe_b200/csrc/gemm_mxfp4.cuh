@@ -188,72 +188,102 @@ __device__ __forceinline__ RowBlock find_block(const GroupTables& t, int G, int 
   return r;
 }
 
+// Two fp32 products (sums) in one instruction, each rounded to nearest.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
 // silu(g) * u = g * u / (1 + 2^(-g log2 e)), in fp32 with the hardware's
 // approximate exponential and reciprocal (2^-22 relative each; the
 // denominator is at least 1, so flushing subnormals changes nothing).
-__device__ __forceinline__ float silu_mul(float g, float u) {
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return g * r * u;
+__device__ __forceinline__ float2 silu_mul2(float2 g, float2 u) {
+  const float2 x = mul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+  float2 e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(x.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(x.y));
+  e = add2(e, make_float2(1.0f, 1.0f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
+  return mul2(mul2(g, r), u);
 }
 
-// 32 output columns of one row, as a warp: quantised to a record's block, or
-// rounded to bf16 and stored as a whole 32 x 32 box by TMA where all 32 rows
-// are the group's, else row by row.
-template <bool QOUT>
-__device__ __forceinline__ void store_chunk(const float (&v)[32], const Params& p,
-                                            const CUtensorMap* tmC, int col0, int64_t row,
-                                            int box_row, bool row_ok, bool box_full, uint32_t stg) {
+// 32 output columns of one row, as a warp: rounded to bf16 and stored as a
+// whole 32 x 32 box by TMA where all 32 rows are the group's, else row by row.
+__device__ __forceinline__ void store_bf16(const float (&v)[32], const Params& p,
+                                           const CUtensorMap* tmC, int col0, int64_t row,
+                                           int box_row, bool row_ok, bool box_full, uint32_t stg) {
   const int lane = threadIdx.x & 31;
-  if constexpr (QOUT) {
-    float m = 0.0f;
+  uint32_t w[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) m = max3_abs(v[2 * i], v[2 * i + 1], m);
-    const uint32_t s = mx_scale_code(__float_as_uint(m));
-    const float inv = mx_inv_scale(s);
-    uint32_t q[4];
+  for (int i = 0; i < 16; ++i) w[i] = cvt_bf16x2(v[2 * i], v[2 * i + 1]);
+  if (box_full) {
+    if (lane == 0) bulk_wait_group_read<0>();
+    __syncwarp();
+    const uint32_t dst = stg + lane * 64;
+    const uint32_t sw = (lane >> 1) & 3;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      q[i] = mx_cvt8(v[8 * i] * inv, v[8 * i + 1] * inv, v[8 * i + 2] * inv, v[8 * i + 3] * inv,
-                     v[8 * i + 4] * inv, v[8 * i + 5] * inv, v[8 * i + 6] * inv,
-                     v[8 * i + 7] * inv);
-    if (row_ok) {
-      const int row_bytes = mx_row_bytes(p.N), cb = mx_code_bytes(p.N), ns = mx_num_scales(p.N);
-      uint8_t* orow = static_cast<uint8_t*>(p.out) + row * row_bytes;
-      *reinterpret_cast<uint4*>(orow + col0 / 2) = make_uint4(q[0], q[1], q[2], q[3]);
-      orow[cb + col0 / 32] = static_cast<uint8_t>(s);
-      if (col0 / 32 == ns - 1)
-        for (int b = cb + ns; b < row_bytes; ++b) orow[b] = 0;
+    for (int c4 = 0; c4 < 4; ++c4)
+      st_shared_v4m(dst + ((c4 ^ sw) << 4),
+                    make_uint4(w[4 * c4], w[4 * c4 + 1], w[4 * c4 + 2], w[4 * c4 + 3]));
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(tmC, col0, box_row, stg);
+      bulk_commit_group();
     }
-  } else {
-    uint32_t w[16];
+  } else if (row_ok) {
+    uint16_t* orow = static_cast<uint16_t*>(p.out) + row * p.N;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = cvt_bf16x2(v[2 * i], v[2 * i + 1]);
-    if (box_full) {
-      if (lane == 0) bulk_wait_group_read<0>();
-      __syncwarp();
-      const uint32_t dst = stg + lane * 64;
-      const uint32_t sw = (lane >> 1) & 3;
-#pragma unroll
-      for (int c4 = 0; c4 < 4; ++c4)
-        st_shared_v4m(dst + ((c4 ^ sw) << 4),
-                      make_uint4(w[4 * c4], w[4 * c4 + 1], w[4 * c4 + 2], w[4 * c4 + 3]));
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        tma_store_2d(tmC, col0, box_row, stg);
-        bulk_commit_group();
-      }
-    } else if (row_ok) {
-      uint16_t* orow = static_cast<uint16_t*>(p.out) + row * p.N;
-#pragma unroll
-      for (int c4 = 0; c4 < 4; ++c4)
-        if (col0 + c4 * 8 + 8 <= p.N)
-          *reinterpret_cast<uint4*>(orow + col0 + c4 * 8) =
-              make_uint4(w[4 * c4], w[4 * c4 + 1], w[4 * c4 + 2], w[4 * c4 + 3]);
-    }
+    for (int c4 = 0; c4 < 4; ++c4)
+      if (col0 + c4 * 8 + 8 <= p.N)
+        *reinterpret_cast<uint4*>(orow + col0 + c4 * 8) =
+            make_uint4(w[4 * c4], w[4 * c4 + 1], w[4 * c4 + 2], w[4 * c4 + 3]);
   }
+}
+
+// A block of 32 values of one row -> its codes and scale.
+__device__ __forceinline__ uint4 quantize_block(const float (&v)[32], uint32_t& s) {
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = max3_abs(v[2 * i], v[2 * i + 1], m);
+  s = mx_scale_code(__float_as_uint(m));
+  const float inv = mx_inv_scale(s);
+  const float2 inv2 = make_float2(inv, inv);
+  uint32_t q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = mul2(make_float2(v[8 * i + 2 * j], v[8 * i + 2 * j + 1]), inv2);
+    q[i] = mx_cvt8(f[0].x, f[0].y, f[1].x, f[1].y, f[2].x, f[2].y, f[3].x, f[3].y);
+  }
+  return make_uint4(q[0], q[1], q[2], q[3]);
+}
+__device__ __forceinline__ uint32_t ld_shared_u8(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
 }
 
 // 32 output columns out of TMEM: 32 accumulator columns, or (SWIGLU) the 32
@@ -269,7 +299,12 @@ __device__ __forceinline__ void load_chunk(uint32_t taddr, float (&v)[32]) {
     tc_wait_ld_regs(ra);
     tc_wait_ld_regs(ua);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = silu_mul(__uint_as_float(ra[i]), __uint_as_float(ua[i]));
+    for (int i = 0; i < 32; i += 2) {
+      const float2 h = silu_mul2(make_float2(__uint_as_float(ra[i]), __uint_as_float(ra[i + 1])),
+                                 make_float2(__uint_as_float(ua[i]), __uint_as_float(ua[i + 1])));
+      v[i] = h.x;
+      v[i + 1] = h.y;
+    }
   } else {
     tc_wait_ld_regs(ra);
 #pragma unroll
@@ -277,25 +312,85 @@ __device__ __forceinline__ void load_chunk(uint32_t taddr, float (&v)[32]) {
   }
 }
 
+// Shared memory of the epilogue: a 2 KiB box per warp (bf16), or per row
+// quadrant two buffers of 32 rows x 48 bytes of codes and 4 of scales.
+constexpr int kQuadBuf = 32 * (16 * kMxTileChunks + 4);
+template <bool QOUT>
+__host__ __device__ constexpr int epi_bytes() {
+  return QOUT ? (4 * 2 * kQuadBuf + 1023) / 1024 * 1024 : kEpiWarps * kEpiBox;
+}
+
 // One CTA's 128 rows of a finished tile, for epilogue warp `w` of kEpiWarps
 // (row quadrant = warp index mod 4; three warps share a quadrant's columns).
-template <bool SWIGLU, bool QOUT>
+// release() is called once by every warp, as soon as it has its last values
+// out of TMEM.
+//
+// Quantised output: a warp holds 32 rows of one block each, and storing those
+// straight from registers touches 32 lines with each instruction (codes and
+// scales: 14 of XL gate_up's 95 us).  So the three warps of a quadrant collect
+// the tile's codes and scales in shared memory and store them row by row, up
+// to 48 bytes a row from neighbouring lanes.  One named barrier a tile (the
+// two buffers alternate); a warp whose wait gave up (`live` false) still goes
+// through it.
+template <bool SWIGLU, bool QOUT, class Release>
 __device__ __forceinline__ void epilogue_tile(const Params& p, const CUtensorMap* tmC, int w,
                                               uint32_t acc_tmem, int row0, int nrows, int chunk0,
-                                              int chunks, uint32_t stg) {
+                                              int chunks, uint32_t epi, int& buf, bool live,
+                                              Release release) {
   const int quad = w & 3, third = w >> 2;
-  if (quad * 32 >= nrows) return;
   const int lane = threadIdx.x & 31;
   const int r = quad * 32 + lane;
-  constexpr int kPer = SWIGLU ? 1 : 2;  // 32-column outputs of a chunk
+  const uint32_t tquad = acc_tmem + (static_cast<uint32_t>(quad * 32) << 16);
+  if (quad * 32 >= nrows) {
+    release();
+    return;
+  }
+  if constexpr (QOUT) {
+    static_assert(SWIGLU && kEpiWarps / 4 >= kMxTileChunks, "a chunk a warp");
+    const uint32_t codes = epi + (quad * 2 + buf) * kQuadBuf;
+    buf ^= 1;  // per tile that the quadrant takes part in: the barrier is between two uses
+    const uint32_t scales = codes + 32 * 16 * kMxTileChunks;
+    if (third < chunks && live) {
+      float v[32];
+      load_chunk<true>(tquad + 64 * third, v);
+      release();
+      uint32_t s;
+      const uint4 q = quantize_block(v, s);
+      st_shared_v4m(codes + lane * (16 * kMxTileChunks) + third * 16, q);
+      asm volatile("st.shared.u8 [%0], %1;" ::"r"(scales + lane * 4 + third), "r"(s) : "memory");
+    } else {
+      release();
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + quad), "n"(8 * kEpiWarps) : "memory");
+    // piece i: 16 bytes of codes, and the scale, of row i / chunks
+    const int i = third * 32 + lane;
+    if (i < 32 * chunks && live) {
+      const int row = chunks == 3 ? i / 3 : chunks == 2 ? i >> 1 : i;
+      const int col = i - row * chunks;
+      const int blk = chunk0 + col;  // block of the output row
+      if (quad * 32 + row < nrows && blk * 32 < p.N) {
+        const int row_bytes = mx_row_bytes(p.N), cb = mx_code_bytes(p.N), ns = mx_num_scales(p.N);
+        uint8_t* orow = static_cast<uint8_t*>(p.out) +
+                        (static_cast<int64_t>(row0) + quad * 32 + row) * row_bytes;
+        *reinterpret_cast<uint4*>(orow + blk * 16) =
+            ld_shared_v4(codes + row * (16 * kMxTileChunks) + col * 16);
+        orow[cb + blk] = static_cast<uint8_t>(ld_shared_u8(scales + row * 4 + col));
+        if (blk == ns - 1)
+          for (int b = cb + ns; b < row_bytes; ++b) orow[b] = 0;
+      }
+    }
+  } else {
+    constexpr int kPer = SWIGLU ? 1 : 2;  // 32-column outputs of a chunk
+    const int end = live ? min(chunks * kPer, cdiv(p.N, 32) - chunk0 * kPer) : 0;
+    if (third >= end) release();
 #pragma unroll 1
-  for (int c = third; c < chunks * kPer; c += kEpiWarps / 4) {
-    const int col0 = (chunk0 * kPer + c) * 32;
-    if (col0 >= p.N) break;
-    float v[32];
-    load_chunk<SWIGLU>(acc_tmem + (static_cast<uint32_t>(quad * 32) << 16) + (SWIGLU ? 64 : 32) * c, v);
-    store_chunk<QOUT>(v, p, tmC, col0, static_cast<int64_t>(row0) + r, row0 + quad * 32, r < nrows,
-                      (quad + 1) * 32 <= nrows, stg);
+    for (int c = third; c < end; c += kEpiWarps / 4) {
+      float v[32];
+      load_chunk<SWIGLU>(tquad + (SWIGLU ? 64 : 32) * c, v);
+      if (c + kEpiWarps / 4 >= end) release();
+      store_bf16(v, p, tmC, (chunk0 * kPer + c) * 32, static_cast<int64_t>(row0) + r,
+                 row0 + quad * 32, r < nrows, (quad + 1) * 32 <= nrows, epi + w * kEpiBox);
+    }
   }
 }
 

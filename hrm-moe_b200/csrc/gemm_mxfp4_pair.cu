@@ -42,7 +42,7 @@ struct Ctl {
   uint64_t a_full[QA], a_empty[QA];
   uint64_t b_full[QB], b_empty[QB];
   uint64_t sf_full[QB];  // the k-block's scales are in TMEM
-  uint64_t raw_full[QR], raw_empty[QR];
+  uint64_t raw_full[QR];
   uint64_t sfa_full[QR], sfa_empty[QR];
   uint64_t acc_full[kAccs], acc_empty[kAccs];
   uint64_t drain;
@@ -57,9 +57,12 @@ constexpr int kOffB = kOffSfa + QR * 2048;
 constexpr int kOffSfb = kOffB + QB * kBBytes;
 constexpr int kOffRaw = kOffSfb + QB * kSfbBytes;  // [128 rows][16 scales]
 constexpr int kOffEpi = kOffRaw + QR * 2048;
-constexpr int kOffCtl = kOffEpi + kEpiWarps * kEpiBox;
-constexpr size_t kSmemBytes = 1024 + kOffCtl + sizeof(Ctl);
-static_assert(kSmemBytes <= 232448, "shared memory budget of one sm_100 CTA");
+template <bool QOUT>
+constexpr int kOffCtl = kOffEpi + epi_bytes<QOUT>();
+template <bool QOUT>
+constexpr size_t kSmemBytes = 1024 + kOffCtl<QOUT> + sizeof(Ctl);
+static_assert(kSmemBytes<false> <= 232448 && kSmemBytes<true> <= 232448,
+              "shared memory budget of one sm_100 CTA");
 
 // Arrive on the leader's barrier: this thread's (and, through the fence, its
 // warp's) shared-memory writes are visible to whoever waits with cluster scope.
@@ -95,6 +98,50 @@ __device__ __forceinline__ bool wait_cluster_bounded(uint32_t bar, uint32_t pari
   }
 }
 
+// The four MMAs of a k-block (accumulating into `d` unless `acc` is 0), with
+// two mbarriers' state asked for in front of them and returned behind them:
+// bit 0 bar0, bit 1 bar1.  One block of PTX, so that nothing waits for the
+// answers in between.  Scale ids 0 and 2 take turns (two scales an MMA, four
+// to a TMEM word); tsfb_step: TMEM columns of B's scales of 128 elements.
+constexpr uint32_t kSfId2 = (2u << 4) | (2u << 29);
+__host__ __device__ constexpr uint64_t smem_desc_sw128_hi() {
+  return (static_cast<uint64_t>(1024u >> 4) << 32) | (static_cast<uint64_t>(1u) << 46) |
+         (static_cast<uint64_t>(2u) << 61);
+}
+__device__ __forceinline__ uint32_t mma_kblock(uint32_t d, uint32_t ad, uint32_t bd, uint32_t id0,
+                                               uint32_t tsfa, uint32_t tsfb, uint32_t tsfb_step,
+                                               uint32_t acc, uint32_t bar0, uint32_t parity0,
+                                               uint32_t bar1, uint32_t parity1) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, t, q0, q1;\n\t"
+      ".reg .b32 id2, sfa2, sfb2, r1, x1, x2, x3, y1, y2, y3;\n\t"
+      ".reg .b64 a0, a1, a2, a3, b0, b1, b2, b3;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 q0, [%9], %10;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 q1, [%11], %12;\n\t"
+      "setp.ne.b32 p, %8, 0;\n\t"
+      "setp.eq.b32 t, %8, %8;\n\t"
+      "or.b32 id2, %4, %13;\n\t"
+      "add.u32 sfa2, %5, 4;\n\tadd.u32 sfb2, %6, %7;\n\t"
+      "add.u32 x1, %2, 2;\n\tadd.u32 x2, %2, 4;\n\tadd.u32 x3, %2, 6;\n\t"
+      "add.u32 y1, %3, 2;\n\tadd.u32 y2, %3, 4;\n\tadd.u32 y3, %3, 6;\n\t"
+      "mov.b64 a0, {%2, %14};\n\tmov.b64 a1, {x1, %14};\n\tmov.b64 a2, {x2, %14};\n\tmov.b64 a3, {x3, %14};\n\t"
+      "mov.b64 b0, {%3, %14};\n\tmov.b64 b1, {y1, %14};\n\tmov.b64 b2, {y2, %14};\n\tmov.b64 b3, {y3, %14};\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%1], a0, b0, %4, [%5], [%6], p;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%1], a1, b1, id2, [%5], [%6], t;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%1], a2, b2, %4, [sfa2], [sfb2], t;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%1], a3, b3, id2, [sfa2], [sfb2], t;\n\t"
+      "selp.u32 %0, 1, 0, q0;\n\t"
+      "selp.u32 r1, 2, 0, q1;\n\t"
+      "or.b32 %0, %0, r1;\n\t}"
+      : "=&r"(r)
+      : "r"(d), "r"(ad), "r"(bd), "r"(id0), "r"(tsfa), "r"(tsfb), "r"(tsfb_step), "r"(acc), "r"(bar0),
+        "r"(parity0), "r"(bar1), "r"(parity1), "n"(kSfId2),
+        "n"(static_cast<uint32_t>(smem_desc_sw128_hi() >> 32))
+      : "memory");
+  return r;
+}
+
 // A unit: a row block and its column tiles [t0, t1).
 struct Unit : RowBlock {
   int t0, t1;
@@ -127,7 +174,7 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  Ctl& ctl = *reinterpret_cast<Ctl*>(smem + kOffCtl);
+  Ctl& ctl = *reinterpret_cast<Ctl*>(smem + kOffCtl<QOUT>);
   const uint32_t sbase = smem_u32(smem);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -150,7 +197,6 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
       }
       for (int s = 0; s < QR; ++s) {
         mbar_init(smem_u32(&ctl.raw_full[s]), 1);
-        mbar_init(smem_u32(&ctl.raw_empty[s]), 1);
         mbar_init(smem_u32(&ctl.sfa_full[s]), 2);   // both CTAs' scale warps
         mbar_init(smem_u32(&ctl.sfa_empty[s]), 1);
       }
@@ -208,25 +254,10 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (elect_one()) {
-      Ring a, b, raw;
+      Ring a, b;
       bool ok = true;
-      const int soff = mx_code_bytes(p.K);
-      // A's scales of k-blocks kb and kb + 1, as the records hold them
-      auto load_raw = [&](int row0, int kb) {
-        if (!mbar_wait_bounded(smem_u32(&ctl.raw_empty[raw.slot]), raw.phase ^ 1u, abort, p.err, lim))
-          return false;
-        const uint32_t fb = smem_u32(&ctl.raw_full[raw.slot]);
-        mbar_arrive_expect_tx(fb, 2048);
-        tma_load_2d(sbase + kOffRaw + raw.slot * 2048, &tmR, soff + kb * 8, row0, fb);
-        raw.next(QR);
-        return true;
-      };
-      Unit un, next;
-      if (pair < units) next = find_unit(ctl, G, p.ct.tiles, pair);
-      if (resident && pair < units)
-        for (int kb = 0; ok && kb < nkb; kb += 2) ok = load_raw(next.row0 + static_cast<int>(rank) * MM, kb);
       for (int u = pair; ok && u < units; u += npairs) {
-        un = next;
+        const Unit un = find_unit(ctl, G, p.ct.tiles, u);
         const int my_row0 = un.row0 + static_cast<int>(rank) * MM;
         for (int t = un.t0; ok && t < un.t1; ++t) {
           const bool longer = t < p.ct.extra;
@@ -238,8 +269,7 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
           const bool load_a = t == un.t0 || !resident;
           for (int kb = 0; kb < nkb; ++kb) {
             if (load_a) {
-              if ((!resident && (kb & 1) == 0 && !load_raw(my_row0, kb)) ||
-                  !mbar_wait_bounded(smem_u32(&ctl.a_empty[a.slot]), a.phase ^ 1u, abort, p.err, lim)) {
+              if (!mbar_wait_bounded(smem_u32(&ctl.a_empty[a.slot]), a.phase ^ 1u, abort, p.err, lim)) {
                 ok = false;
                 break;
               }
@@ -260,18 +290,6 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
             tma_load_2d_pair(sbase + kOffSfb + b.slot * kSfbBytes, mapS, 0, srow + kb * nc, fb_leader);
             b.next(QB);
           }
-          if (ok && t == un.t0 && u + npairs < units) {
-            // the next unit: its scales into the raw ring, its codes into L2
-            // (the loads come in one burst, from every pair, as this unit's
-            // last tile ends)
-            next = find_unit(ctl, G, p.ct.tiles, u + npairs);
-            const int row0 = next.row0 + static_cast<int>(rank) * MM;
-            if (resident)
-              for (int kb = 0; ok && kb < nkb; ++kb) {
-                if ((kb & 1) == 0) ok = load_raw(row0, kb);
-                tma_prefetch_2d(&tmA, kb * kRowB, row0);
-              }
-          }
         }
       }
       // wait until the MMAs have released every slot this CTA filled: no copy
@@ -280,15 +298,25 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
         if (!mbar_wait_bounded(smem_u32(&ctl.a_empty[a.slot]), a.phase ^ 1u, &never, p.err, lim)) break;
       for (int i = 0; i < QB; ++i, b.next(QB))
         if (!mbar_wait_bounded(smem_u32(&ctl.b_empty[b.slot]), b.phase ^ 1u, &never, p.err, lim)) break;
-      for (int i = 0; i < QR; ++i, raw.next(QR))
-        if (!mbar_wait_bounded(smem_u32(&ctl.raw_empty[raw.slot]), raw.phase ^ 1u, &never, p.err, lim)) break;
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
+    // Even a wait on a barrier that is complete takes about 170 cycles here,
+    // two MMAs' time, and the MMA queue is not much longer.  So the state of the
+    // next k-block's barrier, and of the next accumulator's, is asked for in
+    // front of this k-block's MMAs and looked at behind them (mma_kblock).
     if (leader && elect_one()) {
       Ring a, b, acc;
       bool ok = true;
-      const uint64_t adesc0 = smem_desc_sw128(sbase), bdesc0 = smem_desc_sw128(sbase + kOffB);
+      uint32_t ready = 0;  // bit 0: the next k-block, bit 1: the next accumulator
+      // low words of the operands' descriptors (the high words are constant)
+      const uint32_t adesc0 = static_cast<uint32_t>(smem_desc_sw128(sbase));
+      const uint32_t bdesc0 = static_cast<uint32_t>(smem_desc_sw128(sbase + kOffB));
+      const uint32_t a_empty = smem_u32(ctl.a_empty), b_empty = smem_u32(ctl.b_empty);
+      const uint32_t sf_full = smem_u32(ctl.sf_full);
+      const uint32_t acc_full = smem_u32(ctl.acc_full), acc_empty = smem_u32(ctl.acc_empty);
+      const int full_kb = kp / kMxKBlock;           // k-blocks of four MMAs
+      const int tail = cdiv(kp % kMxKBlock, 64);    // MMAs of the last, shorter one
       for (int u = pair; ok && u < units; u += npairs) {
         const Unit un = find_unit(ctl, G, p.ct.tiles, u);
         const int first = a.slot;  // the row block's first slot (resident)
@@ -296,43 +324,49 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
           const int nc = p.ct.count(t);
           const bool load_a = t == un.t0 || !resident;
           const bool free_a = t == un.t1 - 1 || !resident;
-          const uint32_t id0 = idesc_mxf4(2 * MM, 64 * nc, 0), id1 = idesc_mxf4(2 * MM, 64 * nc, 2);
-          if (!mbar_wait_bounded(smem_u32(&ctl.acc_empty[acc.slot]), acc.phase ^ 1u, abort, p.err, lim)) {
+          const uint32_t id0 = idesc_mxf4(2 * MM, 64 * nc, 0);
+          if (!(ready & 2u) &&
+              !mbar_wait_bounded(acc_empty + 8 * acc.slot, acc.phase ^ 1u, abort, p.err, lim)) {
             ok = false;
             break;
           }
-          tc_fence_after();
           const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc.slot * kAccCols);
-          int sa = first;
+          Ring acc_next = acc;
+          acc_next.next(kAccs);
+          const uint32_t next_acc_empty = acc_empty + 8 * acc_next.slot;
+          const uint32_t next_acc_parity = acc_next.phase ^ 1u;
+          int sa = load_a ? a.slot : first;
           for (int kb = 0; kb < nkb; ++kb) {
-            if (load_a) {
-              sa = a.slot;
-              a.next(QA);
-            }
             // committed by a thread that has waited for the k-block's A and B
-            if (!mbar_wait_bounded(smem_u32(&ctl.sf_full[b.slot]), b.phase, abort, p.err, lim)) {
+            if (!(ready & 1u) && !mbar_wait_bounded(sf_full + 8 * b.slot, b.phase, abort, p.err, lim)) {
               ok = false;
               break;
             }
             tc_fence_after();
-            const uint64_t ad = adesc0 + sa * (kABytes >> 4), bd = bdesc0 + b.slot * (kBBytes >> 4);
+            const uint32_t ad = adesc0 + sa * (kABytes >> 4), bd = bdesc0 + b.slot * (kBBytes >> 4);
             const uint32_t tsfa = tmem_base + kSfaCol + kSfaCols * sa;
             const uint32_t tsfb = tmem_base + kSfbCol + kSfbCols * b.slot;
-            const int mmas = min(4, cdiv(kp - kb * kMxKBlock, 64));
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              if (kk >= mmas) break;
-              mma_mxf4_pair(d_tmem, ad + 2 * kk, bd + 2 * kk, (kk & 1) ? id1 : id0,
-                            tsfa + 4 * (kk >> 1), tsfb + 2 * nc * (kk >> 1), (kb | kk) != 0 ? 1u : 0u);
-            }
-            tc_commit_pair_both(smem_u32(&ctl.b_empty[b.slot]));
+            const uint32_t done = b_empty + 8 * b.slot;
             b.next(QB);
-            if (free_a) tc_commit_pair_both(smem_u32(&ctl.a_empty[sa]));
+            if (kb < full_kb) {
+              ready = mma_kblock(d_tmem, ad, bd, id0, tsfa, tsfb, 2 * nc, kb, sf_full + 8 * b.slot,
+                                 b.phase, next_acc_empty, next_acc_parity);
+            } else {
+              constexpr uint64_t kHi = smem_desc_sw128_hi();
+              for (int kk = 0; kk < tail; ++kk)
+                mma_mxf4_pair(d_tmem, kHi | (ad + 2 * kk), kHi | (bd + 2 * kk),
+                              id0 | ((kk & 1) ? kSfId2 : 0u), tsfa + 4 * (kk >> 1),
+                              tsfb + 2 * nc * (kk >> 1), (kb | kk) != 0 ? 1u : 0u);
+              ready = 0;
+            }
+            tc_commit_pair_both(done);
+            if (free_a) tc_commit_pair_both(a_empty + 8 * sa);
+            if (load_a) a.next(QA);
             if (++sa == QA) sa = 0;
           }
           if (!ok) break;
-          tc_commit_pair_both(smem_u32(&ctl.acc_full[acc.slot]));
-          acc.next(kAccs);
+          tc_commit_pair_both(acc_full + 8 * acc.slot);
+          acc = acc_next;
         }
       }
       // every MMA issued has completed, and both CTAs' epilogues have released
@@ -345,10 +379,8 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
     }
   } else if (warp == 3) {
     // ------------------------------------------- scales from shared memory to TMEM
-    // A thread of its own: each tcgen05 instruction takes 40 to 65 cycles to
-    // issue, and copies and MMAs in one thread took longer to issue than the
-    // MMAs to run.  sf_full (commit, mbarrier, fence) hands a k-block on to the
-    // MMA thread.
+    // A thread of its own, so that its waits are not in the MMA thread's way.
+    // sf_full (commit, mbarrier, fence) hands a k-block on to the MMA thread.
     if (leader && elect_one()) {
       Ring a, sa, b;
       bool ok = true;
@@ -401,68 +433,94 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
     // k-blocks at a time, ahead of the codes: the release at cluster scope
     // takes about 900 cycles.  (Loading the scales straight from global memory
     // was slower: the proxy fence waits for the loads in flight behind it.)
-    Ring raw, sa;
-    bool ok = true;
-    for (int u = pair; ok && u < units; u += npairs) {
-      int reps = 1;  // how often the unit's A is loaded
-      if (!resident) {
+    // The warp loads its landing ring itself, QR steps ahead, and asks for the
+    // step's A codes in L2: the units' A loads come in one burst from every
+    // pair when a unit's last tile ends.
+    struct Step {  // two k-blocks of a unit's A
+      int u, rep, kb, row0, reps;
+    };
+    const auto start = [&](Step& st, int u) {
+      st.u = u;
+      st.rep = st.kb = 0;
+      if (u < units) {
         const Unit un = find_unit(ctl, G, p.ct.tiles, u);
-        reps = un.t1 - un.t0;
+        st.row0 = un.row0 + static_cast<int>(rank) * MM;
+        st.reps = resident ? 1 : un.t1 - un.t0;  // how often the unit's A is loaded
       }
-      for (int i = 0; ok && i < reps * cdiv(nkb, 2); ++i) {
-        if (!mbar_wait_bounded(smem_u32(&ctl.raw_full[raw.slot]), raw.phase, abort, p.err, lim)) {
-          ok = false;
-          break;
-        }
-        const uint4* src = reinterpret_cast<const uint4*>(smem + kOffRaw + raw.slot * 2048) + lane;
-        uint4 v[4];
+    };
+    const auto advance = [&](Step& st) {
+      st.kb += 2;
+      if (st.kb >= nkb) {
+        st.kb = 0;
+        if (++st.rep == st.reps) start(st, st.u + npairs);
+      }
+    };
+    const int soff = mx_code_bytes(p.K);
+    Ring in, raw, sa;
+    Step ahead, now;
+    start(ahead, pair);
+    now = ahead;
+    const auto fetch = [&] {
+      if (ahead.u >= units) return;
+      if (elect_one()) {
+        const uint32_t fb = smem_u32(&ctl.raw_full[in.slot]);
+        mbar_arrive_expect_tx(fb, 2048);
+        tma_load_2d(sbase + kOffRaw + in.slot * 2048, &tmR, soff + ahead.kb * 8, ahead.row0, fb);
+        tma_prefetch_2d(&tmA, ahead.kb * kRowB, ahead.row0);
+        if (ahead.kb + 1 < nkb) tma_prefetch_2d(&tmA, (ahead.kb + 1) * kRowB, ahead.row0);
+      }
+      __syncwarp();
+      in.next(QR);
+      advance(ahead);
+    };
+    for (int i = 0; i < QR; ++i) fetch();
+    for (; now.u < units; advance(now)) {
+      if (!mbar_wait_bounded(smem_u32(&ctl.raw_full[raw.slot]), raw.phase, abort, p.err, lim)) break;
+      const uint4* src = reinterpret_cast<const uint4*>(smem + kOffRaw + raw.slot * 2048) + lane;
+      uint4 v[4];
 #pragma unroll
-        for (int h = 0; h < 4; ++h) v[h] = src[32 * h];
-        if (!mbar_wait_bounded(smem_u32(&ctl.sfa_empty[sa.slot]), sa.phase ^ 1u, abort, p.err, lim)) {
-          ok = false;
-          break;
-        }
-        const uint32_t dst = sbase + kOffSfa + sa.slot * 2048 + lane * 16;
-        st_shared_v4m(dst, make_uint4(v[0].x, v[1].x, v[2].x, v[3].x));
-        st_shared_v4m(dst + kAtom, make_uint4(v[0].y, v[1].y, v[2].y, v[3].y));
-        st_shared_v4m(dst + 1024, make_uint4(v[0].z, v[1].z, v[2].z, v[3].z));
-        st_shared_v4m(dst + 1024 + kAtom, make_uint4(v[0].w, v[1].w, v[2].w, v[3].w));
-        fence_proxy_async_smem();
-        __syncwarp();
-        // only here: the stores have taken the values, so the loads are done
-        // (an arrival right behind the loads let the next copy overtake them)
-        if (lane == 0) {
-          mbar_arrive(smem_u32(&ctl.raw_empty[raw.slot]));
-          arrive_release_cluster(map_to_rank(smem_u32(&ctl.sfa_full[sa.slot]), 0));
-        }
-        raw.next(QR);
-        sa.next(QR);
-      }
+      for (int h = 0; h < 4; ++h) v[h] = src[32 * h];
+      if (!mbar_wait_bounded(smem_u32(&ctl.sfa_empty[sa.slot]), sa.phase ^ 1u, abort, p.err, lim)) break;
+      const uint32_t dst = sbase + kOffSfa + sa.slot * 2048 + lane * 16;
+      st_shared_v4m(dst, make_uint4(v[0].x, v[1].x, v[2].x, v[3].x));
+      st_shared_v4m(dst + kAtom, make_uint4(v[0].y, v[1].y, v[2].y, v[3].y));
+      st_shared_v4m(dst + 1024, make_uint4(v[0].z, v[1].z, v[2].z, v[3].z));
+      st_shared_v4m(dst + 1024 + kAtom, make_uint4(v[0].w, v[1].w, v[2].w, v[3].w));
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) arrive_release_cluster(map_to_rank(smem_u32(&ctl.sfa_full[sa.slot]), 0));
+      raw.next(QR);
+      sa.next(QR);
+      // only here may the landing slot be filled again: the stores have taken
+      // the values, so the loads are done
+      fetch();
     }
-    // no commit is on its way to this CTA's barriers when it leaves
+    // no copy into the landing ring is in flight when the CTA leaves (after an
+    // early end), and no commit on its way to its barriers
+    for (; raw.slot != in.slot || raw.phase != in.phase; raw.next(QR))
+      if (!mbar_wait_bounded(smem_u32(&ctl.raw_full[raw.slot]), raw.phase, &never, p.err, lim)) break;
     for (int i = 0; i < QR; ++i, sa.next(QR))
       if (!mbar_wait_bounded(smem_u32(&ctl.sfa_empty[sa.slot]), sa.phase ^ 1u, &never, p.err, lim)) break;
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
     const int w = warp - 4;
-    const uint32_t stg = sbase + kOffEpi + w * kEpiBox;
     Ring acc;
-    bool ok = true;
-    for (int u = pair; ok && u < units; u += npairs) {
+    bool live = true;  // false once a wait gave up: the rest without work
+    int buf = 0;
+    for (int u = pair; u < units; u += npairs) {
       const Unit un = find_unit(ctl, G, p.ct.tiles, u);
       const int my_row0 = un.row0 + static_cast<int>(rank) * MM;
       const int nrows = min(MM, un.row_end - my_row0);  // may be <= 0: nothing to store
       for (int t = un.t0; t < un.t1; ++t) {
-        if (!mbar_wait_bounded(smem_u32(&ctl.acc_full[acc.slot]), acc.phase, abort, p.err, lim)) {
-          ok = false;
-          break;
-        }
+        live = live && mbar_wait_bounded(smem_u32(&ctl.acc_full[acc.slot]), acc.phase, abort, p.err, lim);
         tc_fence_after();
-        epilogue_tile<SWIGLU, QOUT>(p, &tmC, w, tmem_base + acc.slot * kAccCols, my_row0, nrows,
-                                    p.ct.first(t), p.ct.count(t), stg);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&ctl.acc_empty[acc.slot]), 0));
+        epilogue_tile<SWIGLU, QOUT>(
+            p, &tmC, w, tmem_base + acc.slot * kAccCols, my_row0, nrows, p.ct.first(t), p.ct.count(t),
+            sbase + kOffEpi, buf, live, [&] {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&ctl.acc_empty[acc.slot]), 0));
+            });
         acc.next(kAccs);
       }
     }
@@ -488,10 +546,10 @@ cudaError_t launch_variant(unsigned grid, const CUtensorMap& ma, const CUtensorM
   static int done[64] = {0};
   static std::mutex mu;
   const cudaError_t e =
-      allow_smem(grouped_gemm_mxfp4_pair_kernel<SWIGLU, QOUT>, kSmemBytes, done, mu);
+      allow_smem(grouped_gemm_mxfp4_pair_kernel<SWIGLU, QOUT>, kSmemBytes<QOUT>, done, mu);
   if (e != cudaSuccess) return e;
   return launch_pdl(kPdlGemm, grouped_gemm_mxfp4_pair_kernel<SWIGLU, QOUT>, dim3(grid),
-                    dim3(kThreads), kSmemBytes, st, ma, mb, mb1, ms, ms1, mr, mc, p);
+                    dim3(kThreads), kSmemBytes<QOUT>, st, ma, mb, mb1, ms, ms1, mr, mc, p);
 }
 
 }  // namespace
