@@ -1406,7 +1406,6 @@ int mx_validate_shape(const hmoe_shape* s) {
 struct MxExpertBufs {
   DispatchBufs d;
   int32_t* pos;
-  void* xq;   // [T] records of d
   void* xs;   // [A] records of d, by expert
   void* h;    // [A] records of I
   void* out;  // [A, d] bf16: the experts' outputs
@@ -1417,7 +1416,6 @@ MxExpertBufs carve_mx_experts(Carve& c, const hmoe_shape& s) {
   const int64_t A = s.tokens * s.top_k;
   b.d = carve_dispatch(c, s);
   b.pos = c.take<int32_t>(sizeof(int32_t) * A);
-  b.xq = c.take<void>(static_cast<size_t>(mx_row_bytes(s.hidden)) * s.tokens);
   b.xs = c.take<void>(static_cast<size_t>(mx_row_bytes(s.hidden)) * A);
   b.h = c.take<void>(static_cast<size_t>(mx_row_bytes(s.intermediate)) * A);
   b.out = c.take<void>(2 * static_cast<size_t>(s.hidden) * A);
@@ -1441,19 +1439,17 @@ MxFfnBufs carve_mx_ffn(Carve& c, const hmoe_shape& s) {
   return b;
 }
 
-// Quantise (clearing clear_err where it is given), dispatch the records, the
-// two products, combine.
+// Dispatch (the rows become records on the way; reset_err: the error word is
+// cleared first), the two products, combine.
 int run_mx_experts(const hmoe_shape& s, const void* x, const int32_t* idx, const void* w,
                    int w_is_f32, const void* w_gate_up, const void* w_down, const void* final_in,
                    void* out, int32_t* counts_out, int32_t* sort_idx, const MxExpertBufs& b,
-                   int* clear_err, cudaStream_t st) {
+                   bool reset_err, cudaStream_t st) {
   const int64_t A = s.tokens * s.top_k;
-  HMOE_CUDA(launch_mx_quantize(x, s.tokens, s.hidden, s.hidden, s.dtype, b.xq, clear_err, st),
-            "quantize_mxfp4");
-  hmoe_shape rec = s;  // dispatch copies records: rows of 2-byte elements
-  rec.hidden = mx_row_bytes(s.hidden) / 2;
-  int rc = run_dispatch(rec, idx, w, w_is_f32, b.xq, b.d, b.pos, sort_idx, nullptr, nullptr, b.xs, st);
-  if (rc) return rc;
+  HMOE_CUDA(launch_dispatch_mxfp4(idx, x, s.tokens, s.hidden, s.top_k, s.experts, b.d.local_rank,
+                                  b.d.block_counts, b.d.counts, b.pos, sort_idx, b.xs, b.d.err,
+                                  reset_err, st),
+            "dispatch_mxfp4");
   if (counts_out)
     HMOE_CUDA(cudaMemcpyAsync(counts_out, b.d.counts, sizeof(int32_t) * s.experts,
                               cudaMemcpyDeviceToDevice, st), "copy counts");
@@ -1483,8 +1479,7 @@ int hmoe_mxfp4_quantize(const void* x, int64_t rows, int32_t K, int64_t x_stride
     return fail(HMOE_EINVAL, "x, its rows and out must be 16-byte aligned");
   DeviceScope scope;
   if ((rc = select_device(x))) return rc;
-  HMOE_CUDA(launch_mx_quantize(x, rows, K, x_stride, dtype, out, nullptr,
-                               static_cast<cudaStream_t>(stream)),
+  HMOE_CUDA(launch_mx_quantize(x, rows, K, x_stride, dtype, out, static_cast<cudaStream_t>(stream)),
             "quantize_mxfp4");
   return HMOE_OK;
 }
@@ -1530,6 +1525,34 @@ int hmoe_mxfp4_pack_weight(const void* codes, int64_t code_stride, const void* s
   return HMOE_OK;
 }
 
+// The products on a dense x: quantised into `scratch` (M records) first.
+static int mx_grouped_dense(const void* x, int64_t x_stride, int32_t dtype, const void* weight,
+                            const int32_t* tpe, int64_t M, int32_t N, int32_t K, int32_t G,
+                            int swiglu, int quantized_out, void* output, void* scratch,
+                            void* stream) {
+  if (M > 0 && !scratch) return fail(HMOE_EINVAL, "scratch for the quantised rows is required");
+  const int rc = hmoe_mxfp4_quantize(x, M, K, x_stride, dtype, scratch, stream);
+  if (rc) return rc;
+  return mx_grouped(scratch, weight, tpe, M, N, K, G, swiglu, quantized_out, output, nullptr, 0, stream);
+}
+
+int hmoe_grouped_linear_mxfp4_dense(const void* x, int64_t x_stride, int32_t dtype,
+                                    const void* weight, const int32_t* tokens_per_expert,
+                                    int64_t M, int32_t N, int32_t K, int32_t groups, void* output,
+                                    void* scratch, void* stream) {
+  return mx_grouped_dense(x, x_stride, dtype, weight, tokens_per_expert, M, N, K, groups, 0, 0, output,
+                          scratch, stream);
+}
+
+int hmoe_grouped_swiglu_mxfp4_dense(const void* x, int64_t x_stride, int32_t dtype,
+                                    const void* w_gate_up, const int32_t* tokens_per_expert,
+                                    int64_t M, int32_t I, int32_t K, int32_t groups,
+                                    int32_t quantized_out, void* output, void* scratch,
+                                    void* stream) {
+  return mx_grouped_dense(x, x_stride, dtype, w_gate_up, tokens_per_expert, M, I, K, groups, 1,
+                          quantized_out ? 1 : 0, output, scratch, stream);
+}
+
 int hmoe_grouped_linear_mxfp4(const void* rows, const void* weight, const int32_t* tokens_per_expert,
                               int64_t M, int32_t N, int32_t K, int32_t groups, void* output,
                               void* workspace, size_t workspace_bytes, void* stream) {
@@ -1571,7 +1594,7 @@ int hmoe_experts_forward_mxfp4(const hmoe_shape* shape, const void* hidden,
   Carve c{static_cast<char*>(workspace)};
   MxExpertBufs b = carve_mx_experts(c, s);
   return run_mx_experts(s, hidden, topk_idx, topk_weight, 0, w_gate_up, w_down, final_in, y, counts,
-                        sort_idx, b, b.d.err, st);
+                        sort_idx, b, true, st);
 }
 
 size_t hmoe_ffn_mxfp4_workspace_bytes(const hmoe_shape* shape) {
@@ -1604,7 +1627,7 @@ int hmoe_ffn_forward_mxfp4(const hmoe_shape* shape, const void* x, const void* w
                        b.router_scratch, b.x.d.err, st, true),
             "router_topk");
   return run_mx_experts(s, x, idx, b.topk_w, 1, w_gate_up, w_down, accumulate ? y : nullptr, y,
-                        counts, sort_idx, b.x, nullptr, st);
+                        counts, sort_idx, b.x, false, st);
 }
 
 }  // extern "C"

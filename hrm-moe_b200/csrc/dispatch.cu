@@ -17,6 +17,7 @@
 //     its hidden row once and writes it to its k positions.
 #include "common.cuh"
 #include "internal.h"
+#include "mxfp4.cuh"
 
 namespace hmoe {
 namespace {
@@ -212,6 +213,48 @@ __device__ __forceinline__ void copy_row_slice(const uint4* __restrict__ src,
   }
 }
 
+// What a row is on its way to its k positions: copied, or (MX) quantised to an
+// MXFP4 record.  The record form reads x once and writes k records; quantising
+// first and copying records after that took one more kernel and pass.
+enum Payload { kCopy = 0, kMx = 1, kMxWide = 2 };  // kMxWide: d % 32 == 0, 32-byte aligned rows
+
+template <bool WIDE>
+__device__ __forceinline__ void quantize_row_slice(const uint8_t* row, uint8_t* x_sorted, int d,
+                                                   int ncb, int cb, int k, int p, int lane) {
+  const int blocks = mx_num_scales(d), codes = mx_code_bytes(d), row_bytes = mx_row_bytes(d);
+  for (int b0 = cb * 32; b0 < blocks; b0 += ncb * 32) {
+    const int b = b0 + lane;
+    const bool live = b < blocks;
+    uint32_t s = 0;
+    uint4 q = make_uint4(0, 0, 0, 0);
+    if (live) q = mx_quantize_row_block<true, WIDE>(row, b, d, s);
+    for (int j = 0; j < k; ++j) {
+      const int pj = __shfl_sync(0xffffffffu, p, j);
+      if (pj < 0 || !live) continue;
+      uint8_t* dst = x_sorted + static_cast<int64_t>(pj) * row_bytes;
+      reinterpret_cast<uint4*>(dst)[b] = q;
+      dst[codes + b] = static_cast<uint8_t>(s);
+      if (b == blocks - 1)
+        for (int z = codes + blocks; z < row_bytes; ++z) dst[z] = 0;
+    }
+  }
+}
+
+// Token t's row (slice cb of ncb) to its k positions.
+template <int PAYLOAD>
+__device__ __forceinline__ void place_row_slice(const void* x, uint4* x_sorted, int64_t t,
+                                                int row_chunks, int ncb, int cb, int k, int p,
+                                                int lane) {
+  if (PAYLOAD == kCopy)
+    copy_row_slice(static_cast<const uint4*>(x) + t * row_chunks, x_sorted, row_chunks, ncb, cb, k,
+                   p, lane);
+  else  // row_chunks is the row's number of elements
+    quantize_row_slice<PAYLOAD == kMxWide>(static_cast<const uint8_t*>(x) + t * row_chunks * 2,
+                                           reinterpret_cast<uint8_t*>(x_sorted), row_chunks, ncb, cb,
+                                           k, p, lane);
+}
+
+template <int PAYLOAD>
 __global__ void __launch_bounds__(kPermThreads)
 permute_gather_kernel(const int32_t* __restrict__ topk_idx, const int32_t* __restrict__ local_rank,
                       const int32_t* __restrict__ block_offsets, const int32_t* __restrict__ counts,
@@ -245,8 +288,7 @@ permute_gather_kernel(const int32_t* __restrict__ topk_idx, const int32_t* __res
     if (cb == 0) pos[f] = p;
   }
   if (!x_sorted) return;
-  copy_row_slice(static_cast<const uint4*>(x) + t * row_chunks, x_sorted, row_chunks, ncb, cb, k,
-                 p, lane);
+  place_row_slice<PAYLOAD>(x, x_sorted, t, row_chunks, ncb, cb, k, p, lane);
 }
 
 // All of dispatch in one kernel when the T*k assignments fit one histogram
@@ -254,13 +296,14 @@ permute_gather_kernel(const int32_t* __restrict__ topk_idx, const int32_t* __res
 // (the hist_rank computation, repeated per CTA), CTA 0 writes the counts,
 // and each warp then places its slice of a token's row as permute_gather
 // does.  Same positions, one launch instead of two.
+template <int PAYLOAD>
 __global__ void __launch_bounds__(kPermThreads)
 dispatch_small_kernel(const int32_t* __restrict__ topk_idx, const void* __restrict__ topk_w,
                       int topk_w_is_f32, const void* __restrict__ x, int64_t T, int row_chunks,
                       int k, int E, int dtype, int32_t* __restrict__ counts,
                       int32_t* __restrict__ pos, int32_t* __restrict__ sort_idx,
                       int32_t* __restrict__ sorted_token, void* __restrict__ sorted_w,
-                      uint4* __restrict__ x_sorted, int ncb, int* __restrict__ err) {
+                      uint4* __restrict__ x_sorted, int ncb, int* __restrict__ err, int clear_err) {
   static_assert(kPermThreads == kHistThreads, "one histogram pass per CTA");
   __shared__ int32_t cnt[kHistChunks][kMaxExperts];
   __shared__ int32_t rank_s[kHistFlat];
@@ -274,6 +317,10 @@ dispatch_small_kernel(const int32_t* __restrict__ topk_idx, const void* __restri
   grid_dependency_wait();  // launched early (launch_pdl): the routing is written before this
   grid_launch_dependents();
 
+  if (clear_err && blockIdx.x == 0) {  // CTA 0 alone reports in this kernel
+    if (tid == 0) *err = 0;
+    __syncthreads();
+  }
   constexpr int kRounds = kHistChunks / (kHistThreads / 32);
   int my_e[kRounds], my_rank[kRounds];
 #pragma unroll
@@ -354,8 +401,7 @@ dispatch_small_kernel(const int32_t* __restrict__ topk_idx, const void* __restri
     if (cb == 0) pos[f] = p;
   }
   if (!x_sorted) return;
-  copy_row_slice(static_cast<const uint4*>(x) + t * row_chunks, x_sorted, row_chunks, ncb, cb, k,
-                 p, lane);
+  place_row_slice<PAYLOAD>(x, x_sorted, t, row_chunks, ncb, cb, k, p, lane);
 }
 
 __global__ void invert_perm_kernel(const int32_t* __restrict__ sort_idx, int64_t n,
@@ -420,7 +466,7 @@ cudaError_t launch_permute_gather(const int32_t* topk_idx, const int32_t* local_
   // slower for the whole layer)
   const int ncb = T < 512 && x_sorted ? cdiv(row_chunks, 32) : 1;
   const int64_t blocks = cdiv64(T * ncb, kPermThreads / 32);
-  return launch_pdl(kPdlDispatch, permute_gather_kernel, dim3(static_cast<unsigned>(blocks)),
+  return launch_pdl(kPdlDispatch, permute_gather_kernel<kCopy>, dim3(static_cast<unsigned>(blocks)),
                     dim3(kPermThreads), 0, stream, topk_idx, local_rank, block_offsets, counts,
                     topk_w, topk_w_is_f32, x, T, row_chunks, k, E, dispatch_block_tokens(k), dtype,
                     pos, sort_idx, sorted_token, sorted_w, static_cast<uint4*>(x_sorted), ncb);
@@ -438,10 +484,47 @@ cudaError_t launch_dispatch_small(const int32_t* topk_idx, const void* topk_w, i
   const int row_chunks = d * es / 16;
   const int ncb = x_sorted ? cdiv(row_chunks, 32) : 1;
   const int64_t blocks = cdiv64(T * ncb, kPermThreads / 32);
-  return launch_pdl(kPdlDispatch, dispatch_small_kernel, dim3(static_cast<unsigned>(blocks)),
+  return launch_pdl(kPdlDispatch, dispatch_small_kernel<kCopy>, dim3(static_cast<unsigned>(blocks)),
                     dim3(kPermThreads), 0, stream, topk_idx, topk_w, topk_w_is_f32, x, T,
                     row_chunks, k, E, dtype, counts, pos, sort_idx, sorted_token, sorted_w,
-                    static_cast<uint4*>(x_sorted), ncb, err);
+                    static_cast<uint4*>(x_sorted), ncb, err, 0);
+}
+
+namespace {
+bool mx_wide(const void* x, int d) {
+  return d % kMxBlock == 0 && reinterpret_cast<uintptr_t>(x) % 32 == 0;
+}
+}  // namespace
+
+cudaError_t launch_dispatch_mxfp4(const int32_t* topk_idx, const void* x, int64_t T, int d, int k,
+                                  int E, int32_t* local_rank, int32_t* block_counts, int32_t* counts,
+                                  int32_t* pos, int32_t* sort_idx, void* rows_sorted, int* err,
+                                  bool reset_err, cudaStream_t stream) {
+  if (T == 0) return cudaSuccess;
+  if (E > kMaxExperts) return cudaErrorInvalidValue;
+  const bool wide = mx_wide(x, d);
+  // a row over several warps where the tokens alone are too few (as the copy)
+  const bool small = dispatch_fits_one_block(T, k);
+  const int ncb = small || T < 512 ? cdiv(mx_num_scales(d), 32) : 1;
+  const dim3 grid(static_cast<unsigned>(cdiv64(T * ncb, kPermThreads / 32)));
+  uint4* out = static_cast<uint4*>(rows_sorted);
+  if (small)
+    return launch_pdl(kPdlDispatch, wide ? dispatch_small_kernel<kMxWide> : dispatch_small_kernel<kMx>,
+                      grid, dim3(kPermThreads), 0, stream, topk_idx,
+                      static_cast<const void*>(nullptr), 0, x, T, d, k, E, kDtypeBF16, counts, pos,
+                      sort_idx, static_cast<int32_t*>(nullptr), static_cast<void*>(nullptr), out, ncb,
+                      err, reset_err ? 1 : 0);
+  if (reset_err) {
+    const cudaError_t e = cudaMemsetAsync(err, 0, sizeof(int), stream);
+    if (e != cudaSuccess) return e;
+  }
+  const cudaError_t e = launch_hist_scan(topk_idx, T, k, E, local_rank, block_counts, counts, err, stream);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kPdlDispatch, wide ? permute_gather_kernel<kMxWide> : permute_gather_kernel<kMx>,
+                    grid, dim3(kPermThreads), 0, stream, topk_idx, local_rank, block_counts, counts,
+                    static_cast<const void*>(nullptr), 0, x, T, d, k, E, dispatch_block_tokens(k),
+                    kDtypeBF16, pos, sort_idx, static_cast<int32_t*>(nullptr),
+                    static_cast<void*>(nullptr), out, ncb);
 }
 
 cudaError_t launch_invert_perm(const int32_t* sort_idx, int64_t n, int32_t* pos,

@@ -103,6 +103,13 @@ cudaError_t launch_permute_gather(const int32_t* topk_idx, const int32_t* local_
                                   int E, int dtype, int32_t* pos, int32_t* sort_idx,
                                   int32_t* sorted_token, void* sorted_w, void* x_sorted,
                                   cudaStream_t stream);
+// Dispatch whose rows become MXFP4 records on the way: counts, pos, sort_idx
+// (optional) and rows_sorted (records of d) from x [T, d] bf16.  reset_err:
+// *err is cleared first.
+cudaError_t launch_dispatch_mxfp4(const int32_t* topk_idx, const void* x, int64_t T, int d, int k,
+                                  int E, int32_t* local_rank, int32_t* block_counts, int32_t* counts,
+                                  int32_t* pos, int32_t* sort_idx, void* rows_sorted, int* err,
+                                  bool reset_err, cudaStream_t stream);
 // pos[sort_idx[p]] = p for p < n.
 cudaError_t launch_invert_perm(const int32_t* sort_idx, int64_t n, int32_t* pos,
                                cudaStream_t stream);
@@ -238,10 +245,9 @@ cudaError_t launch_colsum_bf16(const void* m, int64_t T, int E, float* partial, 
                                void* out, cudaStream_t stream);
 
 // mxfp4.cu, gemm_mxfp4.cu (layouts: mxfp4.cuh) -----------------------------
-// x [rows, K] (row stride x_stride elements) -> row records.  clear_err (may
-// be null) is set to 0 on the way.
+// x [rows, K] (row stride x_stride elements) -> row records.
 cudaError_t launch_mx_quantize(const void* x, int64_t rows, int K, int64_t x_stride, int dtype,
-                               void* out, int* clear_err, cudaStream_t st);
+                               void* out, cudaStream_t st);
 // Row records -> values [rows, K].
 cudaError_t launch_mx_dequantize(const void* rows_in, int64_t rows, int K, int dtype, void* out,
                                  cudaStream_t st);

@@ -101,4 +101,88 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
   return r;
 }
 
+// Loads of what the kernel before may have written: volatile, and nothing in
+// these kernels is const __restrict__ or __ldg, so that the compiler moves no
+// load above griddepcontrol.wait.
+__device__ __forceinline__ void ld_32bytes(const void* p, uint32_t* w) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]),
+        "=r"(w[7])
+      : "l"(p)
+      : "memory");
+}
+__device__ __forceinline__ uint4 ld_16bytes(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t max_abs_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("{\n\t.reg .b32 x;\n\tabs.bf16x2 x, %2;\n\tmax.NaN.bf16x2 %0, %1, x;\n\t}"
+      : "=r"(r)
+      : "r"(a), "r"(b));
+  return r;
+}
+
+// Block b of a row of K values: codes, and the scale in s.  WIDE: whole blocks,
+// 32-byte aligned rows; else 16-byte loads, each of which may lie behind K (a
+// multiple of 8).
+template <bool BF16, bool WIDE>
+__device__ __forceinline__ uint4 mx_quantize_row_block(const uint8_t* row, int b, int K, uint32_t& s) {
+  constexpr int kWords = BF16 ? 16 : 32;
+  constexpr int ES = BF16 ? 2 : 4;
+  uint32_t w[kWords];
+  const uint8_t* src = row + b * (kMxBlock * ES);
+  if (WIDE) {
+#pragma unroll
+    for (int h = 0; h < kWords / 8; ++h) ld_32bytes(src + 32 * h, w + 8 * h);
+  } else {
+#pragma unroll
+    for (int h = 0; h < kWords / 4; ++h) {
+      const uint4 q = b * kMxBlock + h * (16 / ES) < K ? ld_16bytes(src + 16 * h)
+                                                      : make_uint4(0, 0, 0, 0);
+      w[4 * h] = q.x; w[4 * h + 1] = q.y; w[4 * h + 2] = q.z; w[4 * h + 3] = q.w;
+    }
+  }
+  uint32_t amax;
+  if (BF16) {
+    uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int j = 1; j < 16; ++j) m = max_abs_bf16x2(m, w[j]);
+    amax = max_abs_bf16x2(m, m >> 16) << 16;
+  } else {
+    float m = fabsf(__uint_as_float(w[0]));
+#pragma unroll
+    for (int j = 1; j < 31; j += 2)
+      m = max3_abs(__uint_as_float(w[j % kWords]), __uint_as_float(w[(j + 1) % kWords]), m);
+    amax = __float_as_uint(max3_abs(__uint_as_float(w[kWords - 1]), m, m));
+  }
+  s = mx_scale_code(amax);
+  const float inv = mx_inv_scale(s);
+  uint32_t q[4];
+  if (BF16) {
+    // x / s in bf16: exact (a power of two), or so small that its code is 0
+    const uint32_t inv2 = cvt_bf16x2(inv, inv);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[j] = mul_bf16x2(w[j], inv2);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      q[j] = mx_cvt8(bf16_lo(w[4 * j]), bf16_hi(w[4 * j]), bf16_lo(w[4 * j + 1]),
+                     bf16_hi(w[4 * j + 1]), bf16_lo(w[4 * j + 2]), bf16_hi(w[4 * j + 2]),
+                     bf16_lo(w[4 * j + 3]), bf16_hi(w[4 * j + 3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(w[(8 * j + e) % kWords]) * inv;
+      q[j] = mx_cvt8(f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]);
+    }
+  }
+  return make_uint4(q[0], q[1], q[2], q[3]);
+}
+
 }  // namespace hmoe

@@ -14,6 +14,7 @@ Errors follow the reference: ``ValueError`` for bad shapes
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -490,6 +491,18 @@ class Mxfp4Rows:
         return out
 
 
+def _dense_rows(x: torch.Tensor, code: int):
+    """(x, stride): x with unit stride along its last axis and 16-byte aligned rows."""
+    k = x.shape[-1]
+    if x.dim() == 2 and x.stride(1) == 1:
+        stride = x.stride(0)
+        if stride >= k and stride % (8 if code == _lib.DTYPE_BF16 else 4) == 0 \
+                and x.data_ptr() % 16 == 0:
+            return x, stride
+    x = x.contiguous()
+    return (x if x.data_ptr() % 16 == 0 else x.clone()), k
+
+
 def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Rows:
     """Rows x [..., K] (bf16 or fp32, K a multiple of 8) to MXFP4 along the last axis.
 
@@ -506,17 +519,9 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Rows:
         raise ValueError("quantize_mxfp4 takes rows [..., K]")
     k = shape[-1]
     row_bytes = _mxfp4_row_bytes(k)
-    stride, align = k, 8 if code == _lib.DTYPE_BF16 else 4
-    if len(shape) == 2 and x.stride(1) == 1 and x.stride(0) >= k and x.stride(0) % align == 0:
-        stride = x.stride(0)
-    else:
-        x = x.contiguous()
-    ptr = x.data_ptr()
-    if ptr % 16:
-        x = x.contiguous().clone()
-        ptr, stride = x.data_ptr(), k
+    x, stride = _dense_rows(x, code)
     data = torch.empty((*shape[:-1], row_bytes), dtype=torch.uint8, device=dev)
-    _lib.check(_lib.load().hmoe_mxfp4_quantize(ptr, data.numel() // row_bytes, k, stride, code,
+    _lib.check(_lib.load().hmoe_mxfp4_quantize(x.data_ptr(), data.numel() // row_bytes, k, stride, code,
                                                data.data_ptr(), _raw_stream(dev)))
     return Mxfp4Rows._of(data, k)
 
@@ -593,14 +598,17 @@ def _grouped_mxfp4(what: str, x, weight: Mxfp4Weight, tokens_per_expert: torch.T
     if weight.swiglu != swiglu:
         raise ValueError(f"{what} needs a weight packed with swiglu={swiglu}")
     G, n, k = weight.groups, weight.n, weight.k
-    if not isinstance(x, Mxfp4Rows):
+    dense = not isinstance(x, Mxfp4Rows)
+    if dense:
         if x.requires_grad and torch.is_grad_enabled():
             _refuse_grad(what)
-        if x.dim() == 2 and x.shape[1] != k:
-            raise ValueError(f"grouped GEMM K mismatch: input K={x.shape[1]}, weight K={k}")
-        x = quantize_mxfp4(x)
-    rows = x.data
-    if rows.dim() != 2 or x.k != k:
+        code = dtype_code(x.dtype)
+        rows = x
+        matches = x.dim() == 2 and x.shape[1] == k
+    else:
+        rows = x.data
+        matches = rows.dim() == 2 and x.k == k
+    if not matches:
         raise ValueError(f"grouped GEMM K mismatch: input {tuple(x.shape)}, weight K={k}")
     tpe = tokens_per_expert
     if tpe.numel() != G:
@@ -611,15 +619,26 @@ def _grouped_mxfp4(what: str, x, weight: Mxfp4Weight, tokens_per_expert: torch.T
         tpe = tpe.to(torch.int32).contiguous()
     lib = _lib.load()
     if quantized:
-        out = torch.empty((M, _mxfp4_row_bytes(n)), dtype=torch.uint8, device=dev)
+        out = weight.data.new_empty((M, _mxfp4_row_bytes(n)))
     else:
         out = torch.empty((M, n), dtype=torch.bfloat16, device=dev)
-    args = (rows.data_ptr(), weight.data.data_ptr(), tpe.data_ptr(), M, n, k, G)
-    if swiglu:
-        rc = lib.hmoe_grouped_swiglu_mxfp4(*args, int(quantized), out.data_ptr(), None, 0,
-                                           _raw_stream(dev))
+    if dense:
+        rows, stride = _dense_rows(rows, code)
+        scratch = weight.data.new_empty(M * _mxfp4_row_bytes(k))
+        args = (rows.data_ptr(), stride, code, weight.data.data_ptr(), tpe.data_ptr(), M, n, k, G)
+        if swiglu:
+            rc = lib.hmoe_grouped_swiglu_mxfp4_dense(*args, int(quantized), out.data_ptr(),
+                                                     scratch.data_ptr(), _raw_stream(dev))
+        else:
+            rc = lib.hmoe_grouped_linear_mxfp4_dense(*args, out.data_ptr(), scratch.data_ptr(),
+                                                     _raw_stream(dev))
     else:
-        rc = lib.hmoe_grouped_linear_mxfp4(*args, out.data_ptr(), None, 0, _raw_stream(dev))
+        args = (rows.data_ptr(), weight.data.data_ptr(), tpe.data_ptr(), M, n, k, G)
+        if swiglu:
+            rc = lib.hmoe_grouped_swiglu_mxfp4(*args, int(quantized), out.data_ptr(), None, 0,
+                                               _raw_stream(dev))
+        else:
+            rc = lib.hmoe_grouped_linear_mxfp4(*args, out.data_ptr(), None, 0, _raw_stream(dev))
     _lib.check(rc)
     return Mxfp4Rows._of(out, n) if quantized else out
 
@@ -644,8 +663,20 @@ def grouped_swiglu_mxfp4(x, weight: Mxfp4Weight, tokens_per_expert: torch.Tensor
     return _grouped_mxfp4("grouped_swiglu_mxfp4", x, weight, tokens_per_expert, True, quantized)
 
 
-def _mxfp4_shape(T: int, d: int, dtype: torch.dtype, top_k: int, w_gate_up, w_down,
-                 norm_topk_prob: bool = True) -> _lib.HmoeShape:
+@functools.lru_cache(maxsize=256)
+def _mxfp4_plan(T: int, d: int, E: int, I: int, top_k: int, norm: bool):
+    """(hmoe_shape reference, workspace bytes of the expert call, of the layer call)."""
+    shape = ctypes.byref(make_shape(T, d, E, I, top_k, torch.bfloat16, norm))
+    lib = _lib.load()
+    plan = (shape, lib.hmoe_experts_mxfp4_workspace_bytes(shape),
+            lib.hmoe_ffn_mxfp4_workspace_bytes(shape))
+    if plan[1] == 0 or plan[2] == 0:
+        raise ValueError(_lib.last_error())
+    return plan
+
+
+def _mxfp4_check(T: int, d: int, dtype: torch.dtype, top_k: int, w_gate_up, w_down,
+                 norm_topk_prob: bool = True):
     for w in (w_gate_up, w_down):
         if not isinstance(w, Mxfp4Weight):
             raise TypeError(f"expert weights come from pack_mxfp4_weight, got {type(w).__name__}")
@@ -657,7 +688,7 @@ def _mxfp4_shape(T: int, d: int, dtype: torch.dtype, top_k: int, w_gate_up, w_do
         raise ValueError(
             f"expert weights [{E}, {'2 x ' if w_gate_up.swiglu else ''}{I}, {w_gate_up.k}] / "
             f"[{w_down.groups}, {w_down.n}, {w_down.k}] do not match hidden size {d}")
-    return make_shape(T, d, E, I, top_k, dtype, norm_topk_prob)
+    return _mxfp4_plan(T, d, E, I, top_k, bool(norm_topk_prob))
 
 
 def experts_forward_mxfp4(hidden_states: torch.Tensor, selected_experts: torch.Tensor,
@@ -677,12 +708,12 @@ def experts_forward_mxfp4(hidden_states: torch.Tensor, selected_experts: torch.T
         _refuse_grad("experts_forward_mxfp4")
     T, d = hidden_states.shape
     k = selected_experts.shape[-1]
-    shape = _mxfp4_shape(T, d, hidden_states.dtype, k, w_gate_up, w_down)
+    shape, ws_bytes, _ = _mxfp4_check(T, d, hidden_states.dtype, k, w_gate_up, w_down)
     dev = _require_cuda(hidden_states, selected_experts, routing_weights, final_hidden_states,
                         w_gate_up.data, w_down.data)
     out = final_hidden_states
     if out is None:
-        out = torch.empty((T, d), dtype=torch.bfloat16, device=dev)
+        out = torch.empty_like(hidden_states, memory_format=torch.contiguous_format)
     elif tuple(out.shape) != (T, d) or out.dtype != torch.bfloat16 or not out.is_contiguous():
         raise ValueError(f"final_hidden_states must be contiguous bf16 [{T}, {d}] (it is updated in "
                          "place)")
@@ -698,16 +729,11 @@ def experts_forward_mxfp4(hidden_states: torch.Tensor, selected_experts: torch.T
     if idx.numel() != T * k or rw.numel() != T * k:
         raise ValueError(f"selected_experts {tuple(selected_experts.shape)} and routing_weights "
                          f"{tuple(routing_weights.shape)} do not match {T} tokens")
-    lib = _lib.load()
-    shape = ctypes.byref(shape)
-    ws_bytes = lib.hmoe_experts_mxfp4_workspace_bytes(shape)
-    if ws_bytes == 0:
-        raise ValueError(_lib.last_error())
-    ws = _workspace(ws_bytes, dev)
-    _lib.check(lib.hmoe_experts_forward_mxfp4(
+    ws = w_down.data.new_empty(ws_bytes)
+    _lib.check(_lib.load().hmoe_experts_forward_mxfp4(
         shape, hs.data_ptr(), idx.data_ptr(), rw.data_ptr(), w_gate_up.data.data_ptr(),
         w_down.data.data_ptr(), None if final_hidden_states is None else out.data_ptr(),
-        out.data_ptr(), _ptr(counts_out), _ptr(sort_idx_out), ws.data_ptr(), ws.numel(),
+        out.data_ptr(), _ptr(counts_out), _ptr(sort_idx_out), ws.data_ptr(), ws_bytes,
         _raw_stream(dev)))
     return out
 
@@ -724,7 +750,7 @@ def ffn_forward_mxfp4(x: torch.Tensor, w_router: torch.Tensor, w_gate_up: Mxfp4W
         _refuse_grad("ffn_forward_mxfp4")
     T, d = x.shape
     dt = x.dtype
-    shape = _mxfp4_shape(T, d, dt, top_k, w_gate_up, w_down, norm_topk_prob)
+    shape, _, ws_bytes = _mxfp4_check(T, d, dt, top_k, w_gate_up, w_down, norm_topk_prob)
     E = w_gate_up.groups
     if tuple(w_router.shape) != (E, d):
         raise ValueError(f"router weight is {tuple(w_router.shape)}, expected {(E, d)}")
@@ -747,13 +773,9 @@ def ffn_forward_mxfp4(x: torch.Tensor, w_router: torch.Tensor, w_gate_up: Mxfp4W
             "sort_idx": torch.empty(T * top_k, dtype=torch.int32, device=dev),
         }
     r = routing or {}
-    lib = _lib.load()
-    ws_bytes = lib.hmoe_ffn_mxfp4_workspace_bytes(ctypes.byref(shape))
-    if ws_bytes == 0:
-        raise ValueError(_lib.last_error())
     ws = _workspace(ws_bytes, dev)
-    _lib.check(lib.hmoe_ffn_forward_mxfp4(
-        ctypes.byref(shape), _ptr(x), _ptr(w_router), _ptr(bias), _ptr(w_gate_up.data),
+    _lib.check(_lib.load().hmoe_ffn_forward_mxfp4(
+        shape, _ptr(x), _ptr(w_router), _ptr(bias), _ptr(w_gate_up.data),
         _ptr(w_down.data), _ptr(out), 1 if accumulate else 0, _ptr(r.get("topk_idx")),
         _ptr(r.get("topk_weight")), _ptr(r.get("counts")), _ptr(r.get("sort_idx")), _ptr(ws),
         ws.numel(), _stream(dev)))
@@ -912,7 +934,7 @@ class CapturedFfn:
         E = w_router.shape[0]
         self._mxfp4 = isinstance(w_gate_up, Mxfp4Weight) or isinstance(w_down, Mxfp4Weight)
         if self._mxfp4:
-            self._shape = _mxfp4_shape(T, d, dt, top_k, w_gate_up, w_down, norm_topk_prob)
+            self._shape, _, nbytes = _mxfp4_check(T, d, dt, top_k, w_gate_up, w_down, norm_topk_prob)
             if tuple(w_router.shape) != (w_gate_up.groups, d):
                 raise ValueError(f"router weight is {tuple(w_router.shape)}, expected "
                                  f"{(w_gate_up.groups, d)}")
@@ -924,18 +946,16 @@ class CapturedFfn:
             if tuple(w_gate_up.shape) != (E, 2 * I, d) or tuple(w_down.shape) != (E, d, I):
                 raise ValueError(f"expert weights {tuple(w_gate_up.shape)} / {tuple(w_down.shape)} "
                                  f"do not match hidden size {d} and {E} experts")
-            self._shape = _lib.HmoeShape(T, d, E, I, top_k, dtype_code(dt),
-                                         1 if norm_topk_prob else 0)
+            self._shape = ctypes.byref(_lib.HmoeShape(T, d, E, I, top_k, dtype_code(dt),
+                                                      1 if norm_topk_prob else 0))
+            nbytes = _lib.load().hmoe_ffn_workspace_bytes(self._shape)
+            if nbytes == 0:
+                raise ValueError(_lib.last_error())
             w_gate_up, w_down = w_gate_up.to(dt).contiguous(), w_down.to(dt).contiguous()
         self.x_static = x.detach().clone().contiguous()
         self.y = torch.empty_like(self.x_static)
         self._w = [w_router.to(dt).contiguous(), w_gate_up, w_down,
                    None if router_bias is None else router_bias.to(dt).contiguous()]
-        lib = _lib.load()
-        nbytes = (lib.hmoe_ffn_mxfp4_workspace_bytes if self._mxfp4
-                  else lib.hmoe_ffn_workspace_bytes)(ctypes.byref(self._shape))
-        if nbytes == 0:
-            raise ValueError(_lib.last_error())
         self._ws = _workspace(nbytes, dev)
         self._launch(torch.cuda.current_stream(dev))  # first call: per-device set-up
         torch.cuda.current_stream(dev).synchronize()
@@ -951,7 +971,7 @@ class CapturedFfn:
         lib = _lib.load()
         fn = lib.hmoe_ffn_forward_mxfp4 if self._mxfp4 else lib.hmoe_ffn_forward
         _lib.check(fn(
-            ctypes.byref(self._shape), _ptr(self.x_static), _ptr(wr), _ptr(b), _ptr(wgu), _ptr(wd),
+            self._shape, _ptr(self.x_static), _ptr(wr), _ptr(b), _ptr(wgu), _ptr(wd),
             _ptr(self.y), 0, None, None, None, None, _ptr(self._ws), self._ws.numel(),
             ctypes.c_void_p(stream.cuda_stream)))
 

@@ -432,6 +432,21 @@ int hmoe_grouped_swiglu_mxfp4(const void* rows, const void* w_gate_up,
                               void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * The same two on a dense x [M, K] (bf16 or fp32, x_stride elements from row
+ * to row, rows 16-byte aligned), quantised into `scratch` (M records of K)
+ * first.
+ */
+int hmoe_grouped_linear_mxfp4_dense(const void* x, int64_t x_stride, int32_t dtype,
+                                    const void* weight, const int32_t* tokens_per_expert,
+                                    int64_t M, int32_t N, int32_t K, int32_t groups, void* output,
+                                    void* scratch, void* stream);
+int hmoe_grouped_swiglu_mxfp4_dense(const void* x, int64_t x_stride, int32_t dtype,
+                                    const void* w_gate_up, const int32_t* tokens_per_expert,
+                                    int64_t M, int32_t I, int32_t K, int32_t groups,
+                                    int32_t quantized_out, void* output, void* scratch,
+                                    void* stream);
+
+/*
  * hmoe_experts_forward / hmoe_ffn_forward with packed MXFP4 expert weights
  * (w_gate_up: swiglu = 1, I = intermediate, K = hidden; w_down: swiglu = 0,
  * N = hidden, K = intermediate).  bf16 hidden states, quantised within the
