@@ -19,9 +19,10 @@
 // accumulators of 256 would leave no column for the scales.  A slot's scales
 // live as long as its codes, under the same barriers.
 //
-// The row blocks of all groups, each split into `parts` runs of column tiles,
-// are the units the pairs take in turn; parts is the count that gives the
-// shortest schedule for the actual row counts, found on the device.
+// Work is shared out as whole row blocks, round after round, and the rest as
+// runs of tiles.  (All of it as runs of tiles balanced as well, but the pairs
+// then worked far apart in memory: the down product, bound by its writes,
+// took 117 instead of 92 us.)
 #include "gemm_mxfp4.cuh"
 
 namespace hmoe {
@@ -48,7 +49,6 @@ struct Ctl {
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
-  int parts;
   GroupTables tab;
 };
 
@@ -142,19 +142,49 @@ __device__ __forceinline__ uint32_t mma_kblock(uint32_t d, uint32_t ad, uint32_t
   return r;
 }
 
-// A unit: a row block and its column tiles [t0, t1).
+// A pair's share as a walk over units, a unit being column tiles [t0, t1) of
+// one row block.  Whole rounds first (row blocks pair, pair + npairs, ...: the
+// pairs work side by side on neighbouring rows), then the row blocks left
+// over, their tiles dealt out as runs of equal length.
+struct Walk {
+  int block, blocks_end, step;  // whole row blocks
+  int tile, tile_end;           // the rest
+};
 struct Unit : RowBlock {
   int t0, t1;
 };
-__device__ __forceinline__ Unit find_unit(const Ctl& ctl, int G, int n_tiles, int u) {
-  const int mt = u / ctl.parts;
-  const int part = u - mt * ctl.parts;
-  Unit r;
-  static_cast<RowBlock&>(r) = find_block(ctl.tab, G, mt, 2 * MM);
-  r.t0 = part * n_tiles / ctl.parts;
-  r.t1 = (part + 1) * n_tiles / ctl.parts;
-  return r;
+__device__ __forceinline__ Walk share_of(const Ctl& ctl, int tiles, int pair, int npairs) {
+  const int blocks = ctl.tab.num_m_tiles;
+  const int whole = blocks / npairs * npairs;
+  const int64_t rest = static_cast<int64_t>(blocks - whole) * tiles;
+  Walk w;
+  w.block = pair;
+  w.blocks_end = whole;
+  w.step = npairs;
+  w.tile = whole * tiles + static_cast<int>(rest * pair / npairs);
+  w.tile_end = whole * tiles + static_cast<int>(rest * (pair + 1) / npairs);
+  return w;
 }
+// The walk's next unit; false at its end.
+__device__ __forceinline__ bool next_unit(const Ctl& ctl, int G, int tiles, Walk& w, Unit& un) {
+  int mt;
+  if (w.block < w.blocks_end) {
+    mt = w.block;
+    w.block += w.step;
+    un.t0 = 0;
+    un.t1 = tiles;
+  } else if (w.tile < w.tile_end) {
+    mt = w.tile / tiles;
+    un.t0 = w.tile - mt * tiles;
+    un.t1 = min(tiles, un.t0 + w.tile_end - w.tile);
+    w.tile += un.t1 - un.t0;
+  } else {
+    return false;
+  }
+  static_cast<RowBlock&>(un) = find_block(ctl.tab, G, mt, 2 * MM);
+  return true;
+}
+
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int c0, int c1) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
@@ -218,20 +248,6 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
     __syncwarp();
     grid_dependency_wait();  // launched early (launch_pdl): the counts are written before this
     build_tables(ctl.tab, p.counts, G, p.M, 2 * MM);
-    __syncwarp();
-    if (lane == 0) {
-      // shortest schedule: rounds of units, a unit being its column tiles and
-      // an eighth of one for its own start
-      const int mt = ctl.tab.num_m_tiles;
-      int best = 1;
-      int64_t best_cost = INT64_MAX;
-      for (int parts = 1; parts <= min(p.ct.tiles, 64); ++parts) {
-        const int64_t cost = cdiv64(static_cast<int64_t>(mt) * parts, npairs) *
-                             (8 * cdiv(p.ct.tiles, parts) + 1);
-        if (cost < best_cost) { best_cost = cost; best = parts; }
-      }
-      ctl.parts = best;
-    }
   } else if (warp == 1) {
     tmem_alloc_pair(smem_u32(&ctl.tmem_base), kTmemCols);  // both CTAs, same warp
   }
@@ -243,7 +259,7 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
   grid_launch_dependents();
 
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl.tmem_base, 0);  // uniform, and seen to be
-  const int units = ctl.tab.num_m_tiles * ctl.parts;
+  const Walk share = share_of(ctl, p.ct.tiles, pair, npairs);
   const int kp = mx_padded_k(p.K);
   const int nkb = cdiv(kp, kMxKBlock);
   const bool resident = nkb <= QA;
@@ -256,8 +272,9 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
     if (elect_one()) {
       Ring a, b;
       bool ok = true;
-      for (int u = pair; ok && u < units; u += npairs) {
-        const Unit un = find_unit(ctl, G, p.ct.tiles, u);
+      Walk walk = share;
+      Unit un{};
+      while (ok && next_unit(ctl, G, p.ct.tiles, walk, un)) {
         const int my_row0 = un.row0 + static_cast<int>(rank) * MM;
         for (int t = un.t0; ok && t < un.t1; ++t) {
           const bool longer = t < p.ct.extra;
@@ -317,8 +334,9 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
       const uint32_t acc_full = smem_u32(ctl.acc_full), acc_empty = smem_u32(ctl.acc_empty);
       const int full_kb = kp / kMxKBlock;           // k-blocks of four MMAs
       const int tail = cdiv(kp % kMxKBlock, 64);    // MMAs of the last, shorter one
-      for (int u = pair; ok && u < units; u += npairs) {
-        const Unit un = find_unit(ctl, G, p.ct.tiles, u);
+      Walk walk = share;
+      Unit un{};
+      while (ok && next_unit(ctl, G, p.ct.tiles, walk, un)) {
         const int first = a.slot;  // the row block's first slot (resident)
         for (int t = un.t0; ok && t < un.t1; ++t) {
           const int nc = p.ct.count(t);
@@ -385,8 +403,9 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
       Ring a, sa, b;
       bool ok = true;
       const uint64_t sfa0 = smem_desc_atom(sbase + kOffSfa), sfb0 = smem_desc_atom(sbase + kOffSfb);
-      for (int u = pair; ok && u < units; u += npairs) {
-        const Unit un = find_unit(ctl, G, p.ct.tiles, u);
+      Walk walk = share;
+      Unit un{};
+      while (ok && next_unit(ctl, G, p.ct.tiles, walk, un)) {
         for (int t = un.t0; ok && t < un.t1; ++t) {
           const int nc = p.ct.count(t);
           const bool load_a = t == un.t0 || !resident;
@@ -437,31 +456,32 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
     // step's A codes in L2: the units' A loads come in one burst from every
     // pair when a unit's last tile ends.
     struct Step {  // two k-blocks of a unit's A
-      int u, rep, kb, row0, reps;
+      Walk walk;
+      int rep, kb, row0, reps;
+      bool live;
     };
-    const auto start = [&](Step& st, int u) {
-      st.u = u;
+    const auto start = [&](Step& st) {
+      Unit un{};
+      st.live = next_unit(ctl, G, p.ct.tiles, st.walk, un);
       st.rep = st.kb = 0;
-      if (u < units) {
-        const Unit un = find_unit(ctl, G, p.ct.tiles, u);
-        st.row0 = un.row0 + static_cast<int>(rank) * MM;
-        st.reps = resident ? 1 : un.t1 - un.t0;  // how often the unit's A is loaded
-      }
+      st.row0 = un.row0 + static_cast<int>(rank) * MM;
+      st.reps = resident ? 1 : un.t1 - un.t0;  // how often the unit's A is loaded
     };
     const auto advance = [&](Step& st) {
       st.kb += 2;
       if (st.kb >= nkb) {
         st.kb = 0;
-        if (++st.rep == st.reps) start(st, st.u + npairs);
+        if (++st.rep == st.reps) start(st);
       }
     };
     const int soff = mx_code_bytes(p.K);
     Ring in, raw, sa;
     Step ahead, now;
-    start(ahead, pair);
+    ahead.walk = share;
+    start(ahead);
     now = ahead;
     const auto fetch = [&] {
-      if (ahead.u >= units) return;
+      if (!ahead.live) return;
       if (elect_one()) {
         const uint32_t fb = smem_u32(&ctl.raw_full[in.slot]);
         mbar_arrive_expect_tx(fb, 2048);
@@ -474,7 +494,7 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
       advance(ahead);
     };
     for (int i = 0; i < QR; ++i) fetch();
-    for (; now.u < units; advance(now)) {
+    for (; now.live; advance(now)) {
       if (!mbar_wait_bounded(smem_u32(&ctl.raw_full[raw.slot]), raw.phase, abort, p.err, lim)) break;
       const uint4* src = reinterpret_cast<const uint4*>(smem + kOffRaw + raw.slot * 2048) + lane;
       uint4 v[4];
@@ -507,8 +527,9 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
     Ring acc;
     bool live = true;  // false once a wait gave up: the rest without work
     int buf = 0;
-    for (int u = pair; u < units; u += npairs) {
-      const Unit un = find_unit(ctl, G, p.ct.tiles, u);
+    Walk walk = share;
+    Unit un{};
+    while (next_unit(ctl, G, p.ct.tiles, walk, un)) {
       const int my_row0 = un.row0 + static_cast<int>(rank) * MM;
       const int nrows = min(MM, un.row_end - my_row0);  // may be <= 0: nothing to store
       for (int t = un.t0; t < un.t1; ++t) {
