@@ -75,8 +75,11 @@ __device__ __forceinline__ Tile decode_tile(const GroupTables& tab, const Params
 template <bool SWIGLU, bool QOUT>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
+                          const __grid_constant__ CUtensorMap tmA1,
                           const __grid_constant__ CUtensorMap tmB,
+                          const __grid_constant__ CUtensorMap tmB1,
                           const __grid_constant__ CUtensorMap tmR,
+                          const __grid_constant__ CUtensorMap tmR1,
                           const __grid_constant__ CUtensorMap tmC, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -107,6 +110,7 @@ grouped_gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
       fence_mbar_init();
       tma_prefetch_desc(&tmA);
       tma_prefetch_desc(&tmB);
+      tma_prefetch_desc(&tmB1);
       tma_prefetch_desc(&tmR);
       tma_prefetch_desc(&tmC);
     }
@@ -137,41 +141,53 @@ grouped_gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
     // ------------------------------------------------------------ producer
     if (elect_one()) {
       Ring st, raw;
+      int used = 0, raw_used = 0;
       bool ok = true;
       const int soff = mx_code_bytes(p.K);
       for (int tile = blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
         const Tile t = decode_tile(ctl.tab, p, tile);
-        const int boxes = cdiv(min(MM, t.row_end - t.row0), p.a_box_rows);
+        // A as one box of 128 rows, or the boxes of 32 that the group reaches:
+        // each load costs the producer about 40 cycles, each box the memory
+        // its rows
+        const int nrows = min(MM, t.row_end - t.row0);
+        const bool whole = nrows > MM - 32;
+        const int box = whole ? MM : 32, boxes = whole ? 1 : cdiv(nrows, 32);
+        const CUtensorMap *mapA = whole ? &tmA1 : &tmA, *mapR = whole ? &tmR1 : &tmR;
+        const CUtensorMap* mapB = t.nc > p.ct.chunks ? &tmB1 : &tmB;
         const int brow = t.g * p.b_rows + t.c0 * 64;
         const uint8_t* bs =
             p.b_scales + (static_cast<int64_t>(t.g) * p.b_chunks + t.c0) * nkb * kAtom;
-        // B in boxes of 64 rows
-        const uint32_t bytes = boxes * p.a_box_rows * kRowB + t.nc * (64 * kRowB + kAtom);
+        const uint32_t bytes = boxes * box * kRowB + t.nc * (64 * kRowB + kAtom);
         for (int kb = 0; kb < nkb; ++kb) {
-          if ((kb & 1) == 0) {  // A's scales of two k-blocks
-            if (!wait(ctl.raw_empty[raw.slot], raw.phase ^ 1u)) {
-              ok = false;
-              break;
-            }
-            const uint32_t rb = smem_u32(&ctl.raw_full[raw.slot]);
-            mbar_arrive_expect_tx(rb, boxes * p.a_box_rows * 16);
-            for (int b = 0; b < boxes; ++b)
-              tma_load_2d(sbase + kOffRaw + raw.slot * 2048 + b * p.a_box_rows * 16, &tmR,
-                          soff + kb * 8, t.row0 + b * p.a_box_rows, rb);
-            raw.next(kRaw);
-          }
-          if (!wait(ctl.empty[st.slot], st.phase ^ 1u)) {
+          // the first uses of a stage need no wait (one takes 170 cycles even
+          // when the barrier is complete)
+          if (used < ST) {
+            ++used;
+          } else if (!wait(ctl.empty[st.slot], st.phase ^ 1u)) {
             ok = false;
             break;
           }
           const uint32_t fb = smem_u32(&ctl.full[st.slot]);
           const uint32_t sa = sbase + st.slot * kStageBytes;
           mbar_arrive_expect_tx(fb, bytes);
-          for (int c = 0; c < t.nc; ++c)
-            tma_load_2d(sa + kABytes + c * 64 * kRowB, &tmB, kb * kRowB, brow + c * 64, fb);
+          tma_load_2d(sa + kABytes, mapB, kb * kRowB, brow, fb);
           bulk_load(sa + kOffSfb, bs + static_cast<int64_t>(kb) * t.nc * kAtom, t.nc * kAtom, fb);
           for (int b = 0; b < boxes; ++b)
-            tma_load_2d(sa + b * p.a_box_rows * kRowB, &tmA, kb * kRowB, t.row0 + b * p.a_box_rows, fb);
+            tma_load_2d(sa + b * 32 * kRowB, mapA, kb * kRowB, t.row0 + b * 32, fb);
+          if ((kb & 1) == 0) {  // A's scales of two k-blocks
+            if (raw_used < kRaw) {
+              ++raw_used;
+            } else if (!wait(ctl.raw_empty[raw.slot], raw.phase ^ 1u)) {
+              ok = false;
+              break;
+            }
+            const uint32_t rb = smem_u32(&ctl.raw_full[raw.slot]);
+            mbar_arrive_expect_tx(rb, boxes * box * 16);
+            for (int b = 0; b < boxes; ++b)
+              tma_load_2d(sbase + kOffRaw + raw.slot * 2048 + b * 32 * 16, mapR, soff + kb * 8,
+                          t.row0 + b * 32, rb);
+            raw.next(kRaw);
+          }
           st.next(ST);
         }
       }
@@ -338,8 +354,7 @@ EncodeTiledFn encode_fn() {
 }
 
 template <bool SWIGLU, bool QOUT>
-cudaError_t launch_variant(unsigned grid, const CUtensorMap& ma, const CUtensorMap& mb,
-                           const CUtensorMap& mr, const CUtensorMap& mc, const Params& p,
+cudaError_t launch_variant(unsigned grid, const CUtensorMap (&m)[7], const Params& p,
                            cudaStream_t st) {
   static int done[64] = {0};
   static std::mutex mu;
@@ -347,7 +362,8 @@ cudaError_t launch_variant(unsigned grid, const CUtensorMap& ma, const CUtensorM
       allow_smem(grouped_gemm_mxfp4_kernel<SWIGLU, QOUT>, kSmemBytes<QOUT>, done, mu);
   if (e != cudaSuccess) return e;
   return launch_pdl(kPdlGemm, grouped_gemm_mxfp4_kernel<SWIGLU, QOUT>, dim3(grid), dim3(kThreads),
-                    kSmemBytes<QOUT>, st, ma, mb, mr, mc, p);
+                    kSmemBytes<QOUT>, st, m[0], m[1], m[2], m[3], m[4], m[5], m[6],
+                    p);
 }
 
 }  // namespace
@@ -376,23 +392,26 @@ cudaError_t launch_grouped_gemm_mxfp4(const MxGemmArgs& a, cudaStream_t st) {
   if (forced >= 0 ? forced == 1 : a.M > 192 * static_cast<int64_t>(a.G))
     return launch_grouped_gemm_mxfp4_pair(a, st);
   Params p = make_params(a);
-  p.a_box_rows = a.M > 64 * static_cast<int64_t>(a.G) ? 128 : 32;
   const uint64_t cb = static_cast<uint64_t>(mx_code_bytes(a.K));
-  CUtensorMap ma, mb, mr, mc;
-  if (!make_code_map(&ma, a.rows, static_cast<uint64_t>(a.M), cb, p.a_row_bytes, p.a_box_rows) ||
-      !make_raw_map(&mr, a.rows, static_cast<uint64_t>(a.M), p.a_row_bytes, p.a_box_rows) ||
-      !make_code_map(&mb, a.weight, static_cast<uint64_t>(a.G) * p.b_rows, cb, cb, 64))
+  const uint64_t M = static_cast<uint64_t>(a.M), wrows = static_cast<uint64_t>(a.G) * p.b_rows;
+  CUtensorMap m[7];
+  if (!make_code_map(&m[0], a.rows, M, cb, p.a_row_bytes, 32) ||
+      !make_code_map(&m[1], a.rows, M, cb, p.a_row_bytes, MM) ||
+      !make_code_map(&m[2], a.weight, wrows, cb, cb, 64 * p.ct.chunks) ||
+      !make_code_map(&m[3], a.weight, wrows, cb, cb, 64 * (p.ct.chunks + 1)) ||
+      !make_raw_map(&m[4], a.rows, M, p.a_row_bytes, 32) ||
+      !make_raw_map(&m[5], a.rows, M, p.a_row_bytes, MM))
     return cudaErrorInvalidValue;
   if (a.quantized_out)
-    mc = ma;  // not used
-  else if (!make_out_map(&mc, a.out, static_cast<uint64_t>(a.M), static_cast<uint64_t>(a.N)))
+    m[6] = m[0];  // not used
+  else if (!make_out_map(&m[6], a.out, M, static_cast<uint64_t>(a.N)))
     return cudaErrorInvalidValue;
   const int sms = num_sms_for_current_device();
   const int64_t max_tiles = (cdiv64(a.M, MM) + a.G) * p.ct.tiles;
   const unsigned grid = static_cast<unsigned>(max_tiles < sms ? max_tiles : sms);
-  if (!a.swiglu) return launch_variant<false, false>(grid, ma, mb, mr, mc, p, st);
-  if (a.quantized_out) return launch_variant<true, true>(grid, ma, mb, mr, mc, p, st);
-  return launch_variant<true, false>(grid, ma, mb, mr, mc, p, st);
+  if (!a.swiglu) return launch_variant<false, false>(grid, m, p, st);
+  if (a.quantized_out) return launch_variant<true, true>(grid, m, p, st);
+  return launch_variant<true, false>(grid, m, p, st);
 }
 
 }  // namespace hmoe

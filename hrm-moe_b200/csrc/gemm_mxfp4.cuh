@@ -34,7 +34,6 @@ struct Params {
   int N;            // output columns
   int K;
   int a_row_bytes;
-  int a_box_rows;   // rows of one A load (single-CTA kernel)
   MxColTiles ct;    // column tiles
   int b_rows;       // packed rows per group
   int b_chunks;     // 64-row chunks per group
@@ -140,8 +139,15 @@ __device__ __forceinline__ void build_tables(GroupTables& t, const int32_t* coun
   const int lane = threadIdx.x & 31;
   const int per = cdiv(G, 32);
   const int g0 = min(G, lane * per), g1 = min(G, g0 + per);
+  // up to 128 groups: a lane's counts are loaded at once and kept
+  constexpr int kKeep = 4;
+  int c[kKeep];
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) c[i] = g0 + i < g1 ? max(0, counts[g0 + i]) : 0;
   int64_t rows = 0;
-  for (int g = g0; g < g1; ++g) rows += max(0, counts[g]);
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) rows += c[i];
+  for (int g = g0 + kKeep; g < g1; ++g) rows += max(0, counts[g]);
   int64_t rin = rows;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -150,14 +156,18 @@ __device__ __forceinline__ void build_tables(GroupTables& t, const int32_t* coun
   }
   int64_t rr = rin - rows;
   int tiles = 0;
-  for (int g = g0; g < g1; ++g) {
+  const auto place = [&](int g, int count) {
     const int a = static_cast<int>(rr < M ? rr : M);
-    rr += max(0, counts[g]);
+    rr += count;
     const int b = static_cast<int>(rr < M ? rr : M);
     t.group_rows[g] = a;
     t.tile_prefix[g] = tiles;
     tiles += cdiv(b - a, block_rows);
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i)
+    if (g0 + i < g1) place(g0 + i, c[i]);
+  for (int g = g0 + kKeep; g < g1; ++g) place(g, max(0, counts[g]));
   int tin = tiles;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -430,7 +440,6 @@ inline Params make_params(const MxGemmArgs& a) {
   p.N = a.N;
   p.K = a.K;
   p.a_row_bytes = mx_row_bytes(a.K);
-  p.a_box_rows = MM;
   p.b_rows = mx_weight_rows(a.N, a.swiglu);
   p.b_chunks = cdiv(p.b_rows, 64);
   p.ct = mx_col_tiles(p.b_rows);
