@@ -17,6 +17,10 @@ counts under the reference's keys (models/layers.py:619-632).
 ``SparseMoEGroupedExperts`` under autograd composes the reference's own
 expert steps (layers.py:311-334) around the differentiable grouped GEMM.
 Training is bf16 only, as the reference's Triton backend.
+
+For serving, ``quantize_experts()`` packs the expert weights as MXFP4 next to
+the parameters; inference calls then run the MXFP4 expert products (about a
+quarter of the weight bytes).  Parameters and state dicts are untouched.
 """
 from __future__ import annotations
 
@@ -67,6 +71,12 @@ def _needs_grad(*tensors: Optional[Tensor]) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _refuse_training(*tensors: Optional[Tensor]) -> None:
+    if _needs_grad(*tensors):
+        raise RuntimeError("the experts are quantised to MXFP4, which has no backward: run under "
+                           "torch.no_grad(), or call drop_quantized_experts() to train")
+
+
 def _valid_tokens(total_seqlen, tokens: int) -> int:
     """int(unwrap_tensor(total_seqlen).item()) (models/layers.py:622), at most tokens."""
     v = getattr(total_seqlen, "value", total_seqlen)  # a WrappedTensor holds .value
@@ -92,12 +102,46 @@ class SparseMoEGroupedExperts(nn.Module):
             torch.empty((num_experts, 2 * intermediate_size, hidden_size), **kwargs), init_std_in))
         self.down_weight = nn.Parameter(trunc_normal_(
             torch.empty((num_experts, hidden_size, intermediate_size), **kwargs), init_std_out))
+        self._mxfp4 = None
+
+    def quantize_experts(self) -> None:
+        """Pack both weights as MXFP4 for inference (no counterpart in the reference).
+
+        The packed copies belong to the weights as they are now: after the
+        weights change (an optimizer step, ``load_state_dict``, a move to
+        another device) inference raises until this is called again, or
+        :meth:`drop_quantized_experts` returns to the bf16 products.
+        """
+        self._mxfp4 = (ops.pack_mxfp4_weight(self.gate_up_weight, swiglu=True),
+                       ops.pack_mxfp4_weight(self.down_weight), self._weights_state())
+
+    def drop_quantized_experts(self) -> None:
+        self._mxfp4 = None
+
+    def _weights_state(self):
+        return tuple((w.device, None if w.is_inference() else w._version)
+                     for w in (self.gate_up_weight, self.down_weight))
+
+    def quantized(self):
+        """The packed (gate_up, down) weights, or None.  Refuses stale ones."""
+        if self._mxfp4 is None:
+            return None
+        if self._mxfp4[2] != self._weights_state():
+            raise RuntimeError("the expert weights have changed since quantize_experts(): call it "
+                               "again, or drop_quantized_experts()")
+        return self._mxfp4[:2]
 
     def forward(self, hidden_states: Tensor, selected_experts: Tensor, routing_weights: Tensor,
                 final_hidden_states: Tensor) -> Tensor:
         """Adds the experts' weighted outputs into final_hidden_states (in place)."""
         if hidden_states.shape[0] == 0:
             return final_hidden_states
+        packed = self.quantized()
+        if packed is not None:
+            _refuse_training(hidden_states, routing_weights, self.gate_up_weight, self.down_weight,
+                             final_hidden_states)
+            return ops.experts_forward_mxfp4(hidden_states, selected_experts, routing_weights,
+                                             *packed, final_hidden_states)
         dt = hidden_states.dtype
         w_gate_up, w_down = self.gate_up_weight.to(dt), self.down_weight.to(dt)
         if _needs_grad(hidden_states, routing_weights, w_gate_up, w_down, final_hidden_states):
@@ -158,12 +202,27 @@ class SparseMoESwiGLU(nn.Module):
                                                init_std_in=init_std_in, init_std_out=init_std_out,
                                                **kwargs)
 
+    def quantize_experts(self) -> None:
+        """Serve with MXFP4 expert weights: see SparseMoEGroupedExperts.quantize_experts."""
+        self.experts.quantize_experts()
+
+    def drop_quantized_experts(self) -> None:
+        self.experts.drop_quantized_experts()
+
     def forward(self, x: Tensor, moe_context: Optional[dict[str, Any]] = None,
                 total_seqlen: Optional[Tensor] = None, **_seq_info) -> Tensor:
         original_shape = x.shape
         hidden_states = x.reshape(-1, self.hidden_size)
         dt = hidden_states.dtype
         w_router, bias = self.gate.weight, self.gate.bias
+        packed = self.experts.quantized()
+        if packed is not None:
+            _refuse_training(x, w_router, bias, self.experts.gate_up_weight,
+                             self.experts.down_weight)
+            with torch.no_grad():
+                y = ops.ffn_forward_mxfp4(hidden_states, w_router, *packed, self.top_k,
+                                          self.norm_topk_prob, router_bias=bias)
+            return y.reshape(original_shape)
         w_gate_up = self.experts.gate_up_weight.to(dt)
         w_down = self.experts.down_weight.to(dt)
         # the reference records the aux loss and the expert counts only while

@@ -446,3 +446,68 @@ def test_streams_graphs_and_replays():
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(got, want[700]))
     assert all(torch.equal(a, b) for a, b in zip(other, want[48]))
+
+
+def test_module_with_quantized_experts():
+    ops, L = get_ops(), importlib.import_module("hrm-moe_b200.layers")
+    torch.manual_seed(0)
+    m = L.SparseMoESwiGLU(256, 96, 16, 4, True, router_bias=True, device="cuda", dtype=torch.bfloat16)
+    x = _rand((2, 33, 256), 1)
+    with torch.no_grad():
+        plain = m(x)
+        m.quantize_experts()
+        y = m(x)
+        want = ops.ffn_forward_mxfp4(x.reshape(-1, 256), m.gate.weight,
+                                     ops.pack_mxfp4_weight(m.experts.gate_up_weight, swiglu=True),
+                                     ops.pack_mxfp4_weight(m.experts.down_weight), 4, True,
+                                     router_bias=m.gate.bias)
+        assert y.shape == x.shape and torch.equal(y.reshape(-1, 256), want)
+        # 4-bit operands: each element off by at most a quarter of itself, or an
+        # eighth of the block's scale unit; the products of a layer of three
+        # average that out, and the layers stay recognisably the same
+        rel = (y.double() - plain.double()).norm() / plain.double().norm()
+        assert 0.01 < rel < 0.5
+        # the experts module alone, added into its accumulator
+        idx, rw = ops.router_topk(x.reshape(-1, 256), m.gate.weight, 4, True, m.gate.bias)
+        acc = torch.zeros((66, 256), dtype=torch.bfloat16, device="cuda")
+        got = m.experts(x.reshape(-1, 256), idx, rw, acc)
+        assert got is acc
+        assert torch.equal(acc, ops.experts_forward_mxfp4(x.reshape(-1, 256), idx, rw, *m.experts.quantized()))
+        cap = ops.CapturedFfn(x.reshape(-1, 256), m.gate.weight, *m.experts.quantized(), 4, True, m.gate.bias)
+        assert torch.equal(cap(x.reshape(-1, 256)), want)
+        assert "_mxfp4" not in "".join(m.state_dict())
+        assert m(x[:0]).shape == x[:0].shape
+    with pytest.raises(RuntimeError, match="no backward"):
+        m(x)
+    with torch.no_grad():
+        m.experts.down_weight.mul_(2.0)
+        with pytest.raises(RuntimeError, match="changed"):
+            m(x)
+        m.quantize_experts()
+        assert torch.equal(m(x).double(), 2 * y.double())  # a power of two moves every scale alike
+        m.drop_quantized_experts()
+        assert torch.equal(m(x).double(), 2 * plain.double())
+    m(x).sum().backward()
+    assert m.experts.gate_up_weight.grad is not None
+
+
+def test_refusals_on_the_device():
+    ops = get_ops()
+    x = _rand((8, 64), 1)
+    w = ops.pack_mxfp4_weight(_rand((2, 16, 64), 2))
+    tpe = torch.tensor([4, 4], device="cuda")
+    with pytest.raises(ValueError):
+        ops.quantize_mxfp4(x[:, :20])
+    with pytest.raises(TypeError):
+        ops.grouped_linear_mxfp4(x.half(), w, tpe)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.grouped_linear_mxfp4(x, w, tpe.cpu())
+    with pytest.raises(ValueError, match="even"):
+        ops.pack_mxfp4_weight(_rand((2, 17, 64), 2), swiglu=True)
+    with pytest.raises(ValueError):
+        ops.pack_mxfp4_weight(_rand((2, 20, 64), 2))  # N not a multiple of 8
+    with pytest.raises(ValueError, match="do not match"):
+        ops.experts_forward_mxfp4(x, torch.zeros((8, 1), dtype=torch.int32, device="cuda"),
+                                  torch.ones((8, 1), device="cuda"), w, w)
+    with pytest.raises(TypeError):
+        ops.quantize_mxfp4(x).dequantize(torch.float16)
