@@ -44,11 +44,11 @@ struct Ctl {
 };
 constexpr int kOffRaw = ST * kStageBytes;  // [128 rows][16 scales]
 constexpr int kOffEpi = kOffRaw + kRaw * 2048;
-template <bool QOUT>
-constexpr int kOffCtl = kOffEpi + epi_bytes<QOUT>();
-template <bool QOUT>
-constexpr size_t kSmemBytes = 1024 + kOffCtl<QOUT> + sizeof(Ctl);
-static_assert(kSmemBytes<false> <= 232448 && kSmemBytes<true> <= 232448,
+template <int OUT>
+constexpr int kOffCtl = kOffEpi + epi_bytes<OUT>();
+template <int OUT>
+constexpr size_t kSmemBytes = 1024 + kOffCtl<OUT> + sizeof(Ctl);
+static_assert(kSmemBytes<kBf16> <= 232448 && kSmemBytes<kRecords> <= 232448,
               "shared memory budget of one sm_100 CTA");
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
@@ -72,7 +72,7 @@ __device__ __forceinline__ Tile decode_tile(const GroupTables& tab, const Params
   return t;
 }
 
-template <bool SWIGLU, bool QOUT>
+template <bool SWIGLU, int OUT>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
                           const __grid_constant__ CUtensorMap tmA1,
@@ -84,7 +84,7 @@ grouped_gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  Ctl& ctl = *reinterpret_cast<Ctl*>(smem + kOffCtl<QOUT>);
+  Ctl& ctl = *reinterpret_cast<Ctl*>(smem + kOffCtl<OUT>);
   const uint32_t sbase = smem_u32(smem);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -311,7 +311,7 @@ grouped_gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
       const Tile t = decode_tile(ctl.tab, p, tile);
       live = live && wait(ctl.acc_full[acc.slot], acc.phase);
       tc_fence_after();
-      epilogue_tile<SWIGLU, QOUT>(p, &tmC, w, tmem_base + acc.slot * kAccCols, t.row0,
+      epilogue_tile<SWIGLU, OUT>(p, &tmC, w, tmem_base + acc.slot * kAccCols, t.row0,
                                   min(MM, t.row_end - t.row0), t.c0, t.nc, sbase + kOffEpi, buf, live,
                                   [&] {
                                     tc_fence_before();
@@ -353,16 +353,16 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-template <bool SWIGLU, bool QOUT>
+template <bool SWIGLU, int OUT>
 cudaError_t launch_variant(unsigned grid, const CUtensorMap (&m)[7], const Params& p,
                            cudaStream_t st) {
   static int done[64] = {0};
   static std::mutex mu;
   const cudaError_t e =
-      allow_smem(grouped_gemm_mxfp4_kernel<SWIGLU, QOUT>, kSmemBytes<QOUT>, done, mu);
+      allow_smem(grouped_gemm_mxfp4_kernel<SWIGLU, OUT>, kSmemBytes<OUT>, done, mu);
   if (e != cudaSuccess) return e;
-  return launch_pdl(kPdlGemm, grouped_gemm_mxfp4_kernel<SWIGLU, QOUT>, dim3(grid), dim3(kThreads),
-                    kSmemBytes<QOUT>, st, m[0], m[1], m[2], m[3], m[4], m[5], m[6],
+  return launch_pdl(kPdlGemm, grouped_gemm_mxfp4_kernel<SWIGLU, OUT>, dim3(grid), dim3(kThreads),
+                    kSmemBytes<OUT>, st, m[0], m[1], m[2], m[3], m[4], m[5], m[6],
                     p);
 }
 
@@ -387,9 +387,10 @@ bool make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint
 cudaError_t launch_grouped_gemm_mxfp4(const MxGemmArgs& a, cudaStream_t st) {
   using namespace mx;
   if (a.M == 0 || a.G == 0) return cudaSuccess;
-  if (a.G > kMaxGroups || a.K % 8 != 0 || a.N % 8 != 0) return cudaErrorInvalidValue;
+  if (a.G > kMaxGroups || a.K % 8 != 0 || a.N % 8 != 0 || (a.f32_out && a.swiglu))
+    return cudaErrorInvalidValue;
   const int forced = forced_gemm_kernel();
-  if (forced >= 0 ? forced == 1 : a.M > 192 * static_cast<int64_t>(a.G))
+  if (!a.f32_out && (forced >= 0 ? forced == 1 : a.M > 192 * static_cast<int64_t>(a.G)))
     return launch_grouped_gemm_mxfp4_pair(a, st);
   Params p = make_params(a);
   const uint64_t cb = static_cast<uint64_t>(mx_code_bytes(a.K));
@@ -402,16 +403,17 @@ cudaError_t launch_grouped_gemm_mxfp4(const MxGemmArgs& a, cudaStream_t st) {
       !make_raw_map(&m[4], a.rows, M, p.a_row_bytes, 32) ||
       !make_raw_map(&m[5], a.rows, M, p.a_row_bytes, MM))
     return cudaErrorInvalidValue;
-  if (a.quantized_out)
+  if (a.quantized_out || a.f32_out)
     m[6] = m[0];  // not used
   else if (!make_out_map(&m[6], a.out, M, static_cast<uint64_t>(a.N)))
     return cudaErrorInvalidValue;
   const int sms = num_sms_for_current_device();
   const int64_t max_tiles = (cdiv64(a.M, MM) + a.G) * p.ct.tiles;
   const unsigned grid = static_cast<unsigned>(max_tiles < sms ? max_tiles : sms);
-  if (!a.swiglu) return launch_variant<false, false>(grid, m, p, st);
-  if (a.quantized_out) return launch_variant<true, true>(grid, m, p, st);
-  return launch_variant<true, false>(grid, m, p, st);
+  if (a.f32_out) return launch_variant<false, kF32>(grid, m, p, st);
+  if (!a.swiglu) return launch_variant<false, kBf16>(grid, m, p, st);
+  if (a.quantized_out) return launch_variant<true, kRecords>(grid, m, p, st);
+  return launch_variant<true, kBf16>(grid, m, p, st);
 }
 
 }  // namespace hmoe

@@ -37,7 +37,7 @@ struct Params {
   MxColTiles ct;    // column tiles
   int b_rows;       // packed rows per group
   int b_chunks;     // 64-row chunks per group
-  void* out;        // bf16 [M, N] or records
+  void* out;        // bf16 or fp32 [M, N], or records
   int* err;
   unsigned long long wait_limit_ns;
 };
@@ -322,12 +322,15 @@ __device__ __forceinline__ void load_chunk(uint32_t taddr, float (&v)[32]) {
   }
 }
 
+// What the epilogue writes (kF32: plain product only).
+enum Out { kBf16 = 0, kRecords = 1, kF32 = 2 };
+
 // Shared memory of the epilogue: a 2 KiB box per warp (bf16), or per row
 // quadrant two buffers of 32 rows x 48 bytes of codes and 4 of scales.
 constexpr int kQuadBuf = 32 * (16 * kMxTileChunks + 4);
-template <bool QOUT>
+template <int OUT>
 __host__ __device__ constexpr int epi_bytes() {
-  return QOUT ? (4 * 2 * kQuadBuf + 1023) / 1024 * 1024 : kEpiWarps * kEpiBox;
+  return OUT == kRecords ? (4 * 2 * kQuadBuf + 1023) / 1024 * 1024 : kEpiWarps * kEpiBox;
 }
 
 // One CTA's 128 rows of a finished tile, for epilogue warp `w` of kEpiWarps
@@ -342,7 +345,7 @@ __host__ __device__ constexpr int epi_bytes() {
 // to 48 bytes a row from neighbouring lanes.  One named barrier a tile (the
 // two buffers alternate); a warp whose wait gave up (`live` false) still goes
 // through it.
-template <bool SWIGLU, bool QOUT, class Release>
+template <bool SWIGLU, int OUT, class Release>
 __device__ __forceinline__ void epilogue_tile(const Params& p, const CUtensorMap* tmC, int w,
                                               uint32_t acc_tmem, int row0, int nrows, int chunk0,
                                               int chunks, uint32_t epi, int& buf, bool live,
@@ -355,7 +358,7 @@ __device__ __forceinline__ void epilogue_tile(const Params& p, const CUtensorMap
     release();
     return;
   }
-  if constexpr (QOUT) {
+  if constexpr (OUT == kRecords) {
     static_assert(SWIGLU && kEpiWarps / 4 >= kMxTileChunks, "a chunk a warp");
     const uint32_t codes = epi + (quad * 2 + buf) * kQuadBuf;
     buf ^= 1;  // per tile that the quadrant takes part in: the barrier is between two uses
@@ -398,8 +401,20 @@ __device__ __forceinline__ void epilogue_tile(const Params& p, const CUtensorMap
       float v[32];
       load_chunk<SWIGLU>(tquad + (SWIGLU ? 64 : 32) * c, v);
       if (c + kEpiWarps / 4 >= end) release();
-      store_bf16(v, p, tmC, (chunk0 * kPer + c) * 32, static_cast<int64_t>(row0) + r,
-                 row0 + quad * 32, r < nrows, (quad + 1) * 32 <= nrows, epi + w * kEpiBox);
+      const int col0 = (chunk0 * kPer + c) * 32;
+      if constexpr (OUT == kF32) {
+        if (r < nrows) {
+          float* orow = static_cast<float*>(p.out) + (static_cast<int64_t>(row0) + r) * p.N + col0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (col0 + 4 * i < p.N)  // N is a multiple of 8
+              *reinterpret_cast<float4*>(orow + 4 * i) =
+                  make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        }
+      } else {
+        store_bf16(v, p, tmC, col0, static_cast<int64_t>(row0) + r, row0 + quad * 32, r < nrows,
+                   (quad + 1) * 32 <= nrows, epi + w * kEpiBox);
+      }
     }
   }
 }

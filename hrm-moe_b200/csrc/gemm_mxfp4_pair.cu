@@ -57,11 +57,11 @@ constexpr int kOffB = kOffSfa + QR * 2048;
 constexpr int kOffSfb = kOffB + QB * kBBytes;
 constexpr int kOffRaw = kOffSfb + QB * kSfbBytes;  // [128 rows][16 scales]
 constexpr int kOffEpi = kOffRaw + QR * 2048;
-template <bool QOUT>
-constexpr int kOffCtl = kOffEpi + epi_bytes<QOUT>();
-template <bool QOUT>
-constexpr size_t kSmemBytes = 1024 + kOffCtl<QOUT> + sizeof(Ctl);
-static_assert(kSmemBytes<false> <= 232448 && kSmemBytes<true> <= 232448,
+template <int OUT>
+constexpr int kOffCtl = kOffEpi + epi_bytes<OUT>();
+template <int OUT>
+constexpr size_t kSmemBytes = 1024 + kOffCtl<OUT> + sizeof(Ctl);
+static_assert(kSmemBytes<kBf16> <= 232448 && kSmemBytes<kRecords> <= 232448,
               "shared memory budget of one sm_100 CTA");
 
 // Arrive on the leader's barrier: this thread's (and, through the fence, its
@@ -192,7 +192,7 @@ __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int c0, 
                : "memory");
 }
 
-template <bool SWIGLU, bool QOUT>
+template <bool SWIGLU, int OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
                                const __grid_constant__ CUtensorMap tmB,
@@ -204,7 +204,7 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  Ctl& ctl = *reinterpret_cast<Ctl*>(smem + kOffCtl<QOUT>);
+  Ctl& ctl = *reinterpret_cast<Ctl*>(smem + kOffCtl<OUT>);
   const uint32_t sbase = smem_u32(smem);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -535,7 +535,7 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
       for (int t = un.t0; t < un.t1; ++t) {
         live = live && mbar_wait_bounded(smem_u32(&ctl.acc_full[acc.slot]), acc.phase, abort, p.err, lim);
         tc_fence_after();
-        epilogue_tile<SWIGLU, QOUT>(
+        epilogue_tile<SWIGLU, OUT>(
             p, &tmC, w, tmem_base + acc.slot * kAccCols, my_row0, nrows, p.ct.first(t), p.ct.count(t),
             sbase + kOffEpi, buf, live, [&] {
               tc_fence_before();
@@ -559,7 +559,7 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
   }
 }
 
-template <bool SWIGLU, bool QOUT>
+template <bool SWIGLU, int OUT>
 cudaError_t launch_variant(unsigned grid, const CUtensorMap& ma, const CUtensorMap& mb,
                            const CUtensorMap& mb1, const CUtensorMap& ms, const CUtensorMap& ms1,
                            const CUtensorMap& mr, const CUtensorMap& mc, const Params& p,
@@ -567,10 +567,10 @@ cudaError_t launch_variant(unsigned grid, const CUtensorMap& ma, const CUtensorM
   static int done[64] = {0};
   static std::mutex mu;
   const cudaError_t e =
-      allow_smem(grouped_gemm_mxfp4_pair_kernel<SWIGLU, QOUT>, kSmemBytes<QOUT>, done, mu);
+      allow_smem(grouped_gemm_mxfp4_pair_kernel<SWIGLU, OUT>, kSmemBytes<OUT>, done, mu);
   if (e != cudaSuccess) return e;
-  return launch_pdl(kPdlGemm, grouped_gemm_mxfp4_pair_kernel<SWIGLU, QOUT>, dim3(grid),
-                    dim3(kThreads), kSmemBytes<QOUT>, st, ma, mb, mb1, ms, ms1, mr, mc, p);
+  return launch_pdl(kPdlGemm, grouped_gemm_mxfp4_pair_kernel<SWIGLU, OUT>, dim3(grid),
+                    dim3(kThreads), kSmemBytes<OUT>, st, ma, mb, mb1, ms, ms1, mr, mc, p);
 }
 
 }  // namespace
@@ -598,9 +598,9 @@ cudaError_t launch_grouped_gemm_mxfp4_pair(const MxGemmArgs& a, cudaStream_t st)
   const int64_t max_tiles = (cdiv64(a.M, 2 * MM) + a.G) * p.ct.tiles;
   int pairs = static_cast<int>(max_tiles < sms / 2 ? max_tiles : sms / 2);
   if (pairs < 1) pairs = 1;
-  if (!a.swiglu) return launch_variant<false, false>(2 * pairs, ma, mb, mb1, ms, ms1, mr, mc, p, st);
-  if (a.quantized_out) return launch_variant<true, true>(2 * pairs, ma, mb, mb1, ms, ms1, mr, mc, p, st);
-  return launch_variant<true, false>(2 * pairs, ma, mb, mb1, ms, ms1, mr, mc, p, st);
+  if (!a.swiglu) return launch_variant<false, kBf16>(2 * pairs, ma, mb, mb1, ms, ms1, mr, mc, p, st);
+  if (a.quantized_out) return launch_variant<true, kRecords>(2 * pairs, ma, mb, mb1, ms, ms1, mr, mc, p, st);
+  return launch_variant<true, kBf16>(2 * pairs, ma, mb, mb1, ms, ms1, mr, mc, p, st);
 }
 
 }  // namespace hmoe

@@ -352,15 +352,18 @@ def test_experts_forward(T, d, I, E, k):
     prod[r["sort_idx"].long()] = eo.double()
     prod = prod.reshape(T, k, d) * rw.double()[:, :, None]
     want, mag = prod.sum(1), prod.abs().sum(1)
+    # small calls keep the experts' outputs in fp32: half a bf16 step from `eo`
+    half = BF16 * mag if 4 * T * k * d <= 8 << 20 else torch.zeros_like(mag)
     err = (y.double() - want).abs()
-    assert (err <= BF16 * want.abs() + k * 2.0 ** -23 * mag * (1 + BF16)).all()
+    assert (err <= BF16 * want.abs() + (half + k * 2.0 ** -23 * mag) * (1 + BF16)).all()
     # added into final_hidden_states
     base = _rand((T, d), 9)
     acc = base.clone()
     assert ops.experts_forward_mxfp4(x, idx, rw, pgu, pd, acc) is acc
     want2 = want + base.double()
     err = (acc.double() - want2).abs()
-    assert (err <= BF16 * want2.abs() + (k + 1) * 2.0 ** -23 * (mag + base.double().abs()) * (1 + BF16)).all()
+    assert (err <= BF16 * want2.abs()
+            + (half + (k + 1) * 2.0 ** -23 * (mag + base.double().abs())) * (1 + BF16)).all()
     # against 64 bits: two bf16 roundings, and the codes of h that the fp32 error may move
     xv, gv, dv = _values64(x), _values64(wgu), _values64(wd)
     xs = xv[r["sorted_token"].long()]
