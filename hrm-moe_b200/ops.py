@@ -485,7 +485,7 @@ class Mxfp4Rows:
         code = dtype_code(dtype)
         data, k = self.data, self.k
         dev = _require_cuda(data)
-        out = torch.empty((*data.shape[:-1], k), dtype=dtype, device=dev)
+        out = data.new_empty((*data.shape[:-1], k), dtype=dtype)
         _lib.check(_lib.load().hmoe_mxfp4_dequantize(data.data_ptr(), out.numel() // k, k, code,
                                                      out.data_ptr(), _raw_stream(dev)))
         return out
@@ -520,7 +520,7 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Rows:
     k = shape[-1]
     row_bytes = _mxfp4_row_bytes(k)
     x, stride = _dense_rows(x, code)
-    data = torch.empty((*shape[:-1], row_bytes), dtype=torch.uint8, device=dev)
+    data = x.new_empty((*shape[:-1], row_bytes), dtype=torch.uint8)
     _lib.check(_lib.load().hmoe_mxfp4_quantize(x.data_ptr(), data.numel() // row_bytes, k, stride, code,
                                                data.data_ptr(), _raw_stream(dev)))
     return Mxfp4Rows._of(data, k)
@@ -621,7 +621,7 @@ def _grouped_mxfp4(what: str, x, weight: Mxfp4Weight, tokens_per_expert: torch.T
     if quantized:
         out = weight.data.new_empty((M, _mxfp4_row_bytes(n)))
     else:
-        out = torch.empty((M, n), dtype=torch.bfloat16, device=dev)
+        out = weight.data.new_empty((M, n), dtype=torch.bfloat16)
     if dense:
         rows, stride = _dense_rows(rows, code)
         scratch = weight.data.new_empty(M * _mxfp4_row_bytes(k))
@@ -648,7 +648,8 @@ def grouped_linear_mxfp4(x, weight: Mxfp4Weight, tokens_per_expert: torch.Tensor
 
     ``x`` is :class:`Mxfp4Rows` or a bf16 / fp32 tensor, which is quantised
     first; ``tokens_per_expert`` [G] counts each group's rows, contiguous in
-    order.  Inference only.
+    order.  Rows past the last group are not computed (their output is
+    uninitialised); groups past the last row are cut off.  Inference only.
     """
     return _grouped_mxfp4("grouped_linear_mxfp4", x, weight, tokens_per_expert, False, False)
 

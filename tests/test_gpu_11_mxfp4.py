@@ -281,15 +281,16 @@ def _call_linear(lib, rows, w, tpe, M, out, swiglu=False, quantized=0):
     assert rc == 0, lib.last_error()
 
 
-def test_rows_past_the_groups_and_wrong_counts():
+@pytest.mark.parametrize("M", [300, 1500])  # single CTAs, CTA pairs
+def test_rows_past_the_groups_and_wrong_counts(M):
     ops, lib = get_ops(), importlib.import_module("hrm-moe_b200._lib")
-    M, N, K = 300, 72, 96
+    N, K = 72, 96
     x, w = ops.quantize_mxfp4(_rand((M, K), 1)), ops.pack_mxfp4_weight(_rand((3, N, K), 2, 0.02))
     wg = ops.pack_mxfp4_weight(_rand((3, 2 * N, K), 3, 0.02), swiglu=True)
-    full = torch.tensor([100, 90, 110], dtype=torch.int32, device="cuda")
+    full = torch.tensor([100, 90, M - 190], dtype=torch.int32, device="cuda")
     want = ops.grouped_linear_mxfp4(x, w, full)
-    for counts, done in [([100, 20, 0], 120), ([0, 0, 0], 0), ([100, 90, 2 ** 31 - 1], 300),
-                         ([100, -5, -(2 ** 31)], 100), ([2 ** 31 - 1] * 3, 300)]:
+    for counts, done in [([100, 20, 0], 120), ([0, 0, 0], 0), ([100, 90, 2 ** 31 - 1], M),
+                         ([100, -5, -(2 ** 31)], 100), ([2 ** 31 - 1] * 3, M)]:
         tpe = torch.tensor(counts, dtype=torch.int32, device="cuda")
         out = torch.full((M, N), 7.0, dtype=torch.bfloat16, device="cuda")
         _call_linear(lib, x, w, tpe, M, out)
@@ -379,6 +380,57 @@ def test_experts_forward(T, d, I, E, k):
     ytol = (lim.reshape(T, k, d) * rw.double()[:, :, None]).sum(1)
     ytol = (ytol + k * 2.0 ** -23 * mag) * (1 + BF16) + BF16 * y64.abs()
     assert ((y.double() - y64).abs() <= ytol).all()
+
+
+def test_rows_aligned_to_16_bytes_only():
+    """Inputs, accumulators and weights that start 16 bytes past a 32-byte boundary."""
+    ops = get_ops()
+    T, d, I, E, k = 70, 96, 64, 4, 2
+    x, idx, rw, wgu, wd = _layer(T, d, I, E, k, 8)
+    pgu, pd = ops.pack_mxfp4_weight(wgu, swiglu=True), ops.pack_mxfp4_weight(wd)
+    want = ops.experts_forward_mxfp4(x, idx, rw, pgu, pd)
+
+    def shifted(t):
+        buf = torch.empty(t.numel() + 16, dtype=t.dtype, device="cuda")
+        off = 16 // t.element_size()
+        out = buf[off:off + t.numel()].view(t.shape)
+        assert out.data_ptr() % 32 == 16
+        return out.copy_(t)
+
+    for dt in (torch.bfloat16, torch.float32):
+        assert torch.equal(ops.quantize_mxfp4(shifted(x.to(dt))).data, ops.quantize_mxfp4(x.to(dt)).data)
+    acc = shifted(torch.zeros_like(x))
+    got = ops.experts_forward_mxfp4(shifted(x), idx, rw, ops.pack_mxfp4_weight(shifted(wgu), swiglu=True),
+                                    pd, acc)
+    assert torch.equal(got, want)
+
+
+def test_error_word_of_the_expert_call():
+    """Expert ids outside [0, E) are reported in the workspace's error word, and the next
+    call on the workspace clears it (both dispatch forms)."""
+    ops, lib = get_ops(), importlib.import_module("hrm-moe_b200._lib")
+    d, I, E, k = 64, 32, 8, 2
+    for T in (40, 900):
+        x, idx, rw, wgu, wd = _layer(T, d, I, E, k, T)
+        pgu, pd = ops.pack_mxfp4_weight(wgu, swiglu=True), ops.pack_mxfp4_weight(wd)
+        so, shape = lib.load(), lib.HmoeShape(T, d, E, I, k, 0, 1)
+        ws = torch.empty(so.hmoe_experts_mxfp4_workspace_bytes(ctypes.byref(shape)), dtype=torch.uint8,
+                         device="cuda")
+        y = torch.empty_like(x)
+        p = lambda t: ctypes.c_void_p(t.data_ptr())
+        for bad in (True, False):
+            ids = idx.clone()
+            if bad:
+                ids[3, 1] = E
+            rc = so.hmoe_experts_forward_mxfp4(
+                ctypes.byref(shape), p(x), p(ids), p(rw), p(pgu.data), p(pd.data), None, p(y), None,
+                None, p(ws), ws.numel(), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+            assert rc == 0, lib.last_error()
+            if bad:
+                with pytest.raises(ValueError):
+                    ops.workspace_status(ws)
+            else:
+                ops.workspace_status(ws)
 
 
 def test_experts_forward_drops_and_empty():
