@@ -511,6 +511,9 @@ class SparseMoEExpertParallelSwiGLU(torch.nn.Module):
     def forward(self, x, moe_context=None, total_seqlen=None, **_seq_info):
         from .layers import _needs_grad, _valid_tokens
         le = self.experts.local_experts
+        if le.quantized() is not None:
+            raise RuntimeError("the expert-parallel layer has no MXFP4 form: call "
+                               "drop_quantized_experts() on its local experts")
         want_aux = moe_context is not None and torch.is_grad_enabled()
         if want_aux or _needs_grad(x, self.gate.weight, le.gate_up_weight, le.down_weight):
             # training: the differentiable NCCL orchestration (either transport)

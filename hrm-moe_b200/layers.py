@@ -113,14 +113,17 @@ class SparseMoEGroupedExperts(nn.Module):
         :meth:`drop_quantized_experts` returns to the bf16 products.
         """
         self._mxfp4 = (ops.pack_mxfp4_weight(self.gate_up_weight, swiglu=True),
-                       ops.pack_mxfp4_weight(self.down_weight), self._weights_state())
+                       ops.pack_mxfp4_weight(self.down_weight), self._weights_state(),
+                       (self.gate_up_weight, self.down_weight))  # kept: their ids stay theirs
 
     def drop_quantized_experts(self) -> None:
         self._mxfp4 = None
 
     def _weights_state(self):
-        return tuple((w.device, None if w.is_inference() else w._version)
-                     for w in (self.gate_up_weight, self.down_weight))
+        # the parameter itself, its storage and its version: another parameter
+        # or .data in its place counts as a change too
+        return [(id(w), w.device, w.data_ptr(), None if w.is_inference() else w._version)
+                for w in (self.gate_up_weight, self.down_weight)]
 
     def quantized(self):
         """The packed (gate_up, down) weights, or None.  Refuses stale ones."""
@@ -219,6 +222,9 @@ class SparseMoESwiGLU(nn.Module):
         if packed is not None:
             _refuse_training(x, w_router, bias, self.experts.gate_up_weight,
                              self.experts.down_weight)
+            if moe_context is not None and torch.is_grad_enabled():
+                raise RuntimeError("the experts are quantised to MXFP4, which records no aux loss: "
+                                   "run under torch.no_grad(), or without a moe_context")
             with torch.no_grad():
                 y = ops.ffn_forward_mxfp4(hidden_states, w_router, *packed, self.top_k,
                                           self.norm_topk_prob, router_bias=bias)

@@ -719,7 +719,14 @@ def experts_forward_mxfp4(hidden_states: torch.Tensor, selected_experts: torch.T
     elif tuple(out.shape) != (T, d) or out.dtype != torch.bfloat16 or not out.is_contiguous():
         raise ValueError(f"final_hidden_states must be contiguous bf16 [{T}, {d}] (it is updated in "
                          "place)")
+    for what, t, n in (("counts_out", counts_out, w_gate_up.groups),
+                       ("sort_idx_out", sort_idx_out, T * k)):
+        if t is not None and (t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous()
+                              or t.device != dev):
+            raise ValueError(f"{what} must be {n} contiguous int32 on {dev}")
     if T == 0:
+        if counts_out is not None:
+            counts_out.zero_()
         return out
     hs, idx, rw = hidden_states, selected_experts, routing_weights
     if not hs.is_contiguous():

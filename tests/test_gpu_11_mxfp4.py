@@ -566,3 +566,16 @@ def test_refusals_on_the_device():
                                   torch.ones((8, 1), device="cuda"), w, w)
     with pytest.raises(TypeError):
         ops.quantize_mxfp4(x).dequantize(torch.float16)
+    gu = ops.pack_mxfp4_weight(_rand((2, 16, 64), 3), swiglu=True)
+    dn = ops.pack_mxfp4_weight(_rand((2, 64, 8), 4))
+    idx, rw = torch.zeros((8, 1), dtype=torch.int32, device="cuda"), torch.ones((8, 1), device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for bad in ({"counts_out": torch.zeros(1, **i32)}, {"counts_out": torch.zeros(2, device="cuda")},
+                {"sort_idx_out": torch.zeros(7, **i32)}, {"sort_idx_out": torch.zeros(16, **i32)[::2]}):
+        with pytest.raises(ValueError, match="contiguous int32"):
+            ops.experts_forward_mxfp4(x, idx, rw, gu, dn, **bad)
+    counts, order = torch.full((2,), -1, **i32), torch.full((8,), -1, **i32)
+    ops.experts_forward_mxfp4(x, idx, rw, gu, dn, counts_out=counts, sort_idx_out=order)
+    assert counts.tolist() == [8, 0] and order.tolist() == list(range(8))
+    ops.experts_forward_mxfp4(x[:0], idx[:0], rw[:0], gu, dn, counts_out=counts)
+    assert counts.tolist() == [0, 0]

@@ -153,3 +153,33 @@ def test_python_refusals_without_a_gpu(ops):
         ops.ffn_forward_mxfp4(x, torch.zeros(2, 64), torch.zeros(2, 64, 64), down, 1, True)
     with pytest.raises(RuntimeError, match="inference"):
         ops.ffn_forward_mxfp4(x, torch.zeros(2, 64, requires_grad=True), up, down, 1, True)
+
+
+def test_modules_refuse_stale_and_unserved_quantised_experts(ops):
+    """What the modules refuse before any kernel; the packed weights stand in as strings."""
+    layers = importlib.import_module("hrm-moe_b200.layers")
+    ep = importlib.import_module("hrm-moe_b200.ep")
+
+    def quantised(experts):
+        experts._mxfp4 = ("gate_up", "down", experts._weights_state(),
+                          (experts.gate_up_weight, experts.down_weight))
+        return experts
+
+    m = layers.SparseMoESwiGLU(32, 16, 4, 2, True, dtype=torch.bfloat16).requires_grad_(False)
+    assert quantised(m.experts).quantized() == ("gate_up", "down")
+    with pytest.raises(RuntimeError, match="no aux loss"):
+        m(torch.zeros(3, 32, dtype=torch.bfloat16), moe_context={})
+    w = m.experts.down_weight
+    w.data = w.data.clone()  # leaves the version as it was
+    with pytest.raises(RuntimeError, match="changed"):
+        m(torch.zeros(3, 32, dtype=torch.bfloat16))
+    quantised(m.experts).gate_up_weight = torch.nn.Parameter(m.experts.gate_up_weight.clone())
+    with pytest.raises(RuntimeError, match="changed"):
+        m.experts.quantized()
+    m.drop_quantized_experts()
+    assert m.experts.quantized() is None
+
+    e = ep.SparseMoEExpertParallelSwiGLU(32, 16, 4, 2, True, dtype=torch.bfloat16)
+    quantised(e.experts.local_experts)
+    with pytest.raises(RuntimeError, match="no MXFP4 form"):
+        e(torch.zeros(3, 32, dtype=torch.bfloat16))
