@@ -8,6 +8,9 @@ Python host side.
     layers.SparseMoESwiGLU(..., implementation="grouped_b200")
     ops.ffn_forward / router_topk / dispatch / grouped_linear /
         grouped_swiglu / combine / experts_forward
+    ops.quantize_mxfp4 / pack_mxfp4_weight / grouped_linear_mxfp4 /
+        grouped_swiglu_mxfp4 / experts_forward_mxfp4 / ffn_forward_mxfp4
+        (4-bit microscaled expert weights, inference)
     torch_ops: torch.ops.hrm_moe.ffn_forward / grouped_linear
     ep.PeerExpertParallel / ep.ep_forward (expert parallelism)
 """

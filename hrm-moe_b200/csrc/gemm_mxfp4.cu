@@ -13,6 +13,11 @@
 // brings A's scales into the atom layout; warp 3 copies the atoms to TMEM;
 // warp 1 issues the MMAs; twelve warps run the epilogue.  Each stage has its
 // own TMEM scale columns, so a stage's empty barrier covers its scales as well.
+//
+// Such calls read each expert's weights once: XL 64x8 at T=64 53.5 MB for
+// gate_up, 15.6 us, and 26.7 MB for down, 14.5 us (about half of each is the
+// launch, the group tables and the first tile's way through the pipeline,
+// 8 us for a single tile).
 #include "gemm_mxfp4.cuh"
 
 namespace hmoe {
