@@ -1403,20 +1403,12 @@ int mx_validate_shape(const hmoe_shape* s) {
   return mx_check_weight(s->experts, s->hidden, s->intermediate, 0);
 }
 
-// The experts' outputs wait for the combine in bf16, or in fp32 while that is
-// at most 8 MiB: the extra bytes stay in L2 (64 tokens of XL, 3 MiB: 1 us of
-// 31), and the result's error is that of its own rounding.  Through bf16 it is
-// 1.4 times that on average, and for a few tokens what chance makes of it.
-bool mx_f32_rows(const hmoe_shape& s) {
-  return 4 * s.tokens * s.top_k * static_cast<int64_t>(s.hidden) <= (8ll << 20);
-}
-
 struct MxExpertBufs {
   DispatchBufs d;
   int32_t* pos;
   void* xs;   // [A] records of d, by expert
   void* h;    // [A] records of I
-  void* out;  // [A, d] bf16 or fp32: the experts' outputs
+  float* out;  // [A, d]: the experts' outputs, as the products summed them
 };
 
 MxExpertBufs carve_mx_experts(Carve& c, const hmoe_shape& s) {
@@ -1426,7 +1418,7 @@ MxExpertBufs carve_mx_experts(Carve& c, const hmoe_shape& s) {
   b.pos = c.take<int32_t>(sizeof(int32_t) * A);
   b.xs = c.take<void>(static_cast<size_t>(mx_row_bytes(s.hidden)) * A);
   b.h = c.take<void>(static_cast<size_t>(mx_row_bytes(s.intermediate)) * A);
-  b.out = c.take<void>((mx_f32_rows(s) ? 4 : 2) * static_cast<size_t>(s.hidden) * A);
+  b.out = c.take<float>(sizeof(float) * static_cast<size_t>(s.hidden) * A);
   return b;
 }
 
@@ -1464,9 +1456,9 @@ int run_mx_experts(const hmoe_shape& s, const void* x, const int32_t* idx, const
   MxGemmArgs gu{b.xs, w_gate_up, b.d.counts, b.h, A, s.intermediate, s.hidden, s.experts, 1, 1, b.d.err};
   HMOE_CUDA(launch_grouped_gemm_mxfp4(gu, st), "grouped_swiglu_mxfp4");
   MxGemmArgs dn{b.h, w_down, b.d.counts, b.out, A, s.hidden, s.intermediate, s.experts, 0, 0, b.d.err};
-  dn.f32_out = mx_f32_rows(s) ? 1 : 0;
+  dn.f32_out = 1;
   HMOE_CUDA(launch_grouped_gemm_mxfp4(dn, st), "grouped_linear_mxfp4");
-  HMOE_CUDA(launch_combine_f32(b.out, dn.f32_out, b.pos, w, w_is_f32, s.tokens, s.hidden, s.top_k, final_in, out,
+  HMOE_CUDA(launch_combine_f32(b.out, b.pos, w, w_is_f32, s.tokens, s.hidden, s.top_k, final_in, out,
                                st), "combine");
   return HMOE_OK;
 }

@@ -1,6 +1,6 @@
 // Grouped GEMM by expert on MXFP4 operands: block-scaled tcgen05 MMAs
 // (kind::mxf4, K = 64, one e8m0 scale per 32), fp32 accumulation in TMEM.
-//   plain:   out[rows of g] = x[rows of g] @ w[g]^T               -> bf16
+//   plain:   out[rows of g] = x[rows of g] @ w[g]^T               -> bf16 or fp32
 //   SwiGLU:  h = silu(x @ gate^T) * (x @ up^T), in fp32           -> bf16 or
 //            MXFP4 records (the next product's input; h never exists in bf16)
 //
@@ -395,7 +395,7 @@ cudaError_t launch_grouped_gemm_mxfp4(const MxGemmArgs& a, cudaStream_t st) {
   if (a.G > kMaxGroups || a.K % 8 != 0 || a.N % 8 != 0 || (a.f32_out && a.swiglu))
     return cudaErrorInvalidValue;
   const int forced = forced_gemm_kernel();
-  if (!a.f32_out && (forced >= 0 ? forced == 1 : a.M > 192 * static_cast<int64_t>(a.G)))
+  if (forced >= 0 ? forced == 1 : a.M > 192 * static_cast<int64_t>(a.G))
     return launch_grouped_gemm_mxfp4_pair(a, st);
   Params p = make_params(a);
   const uint64_t cb = static_cast<uint64_t>(mx_code_bytes(a.K));
@@ -408,9 +408,9 @@ cudaError_t launch_grouped_gemm_mxfp4(const MxGemmArgs& a, cudaStream_t st) {
       !make_raw_map(&m[4], a.rows, M, p.a_row_bytes, 32) ||
       !make_raw_map(&m[5], a.rows, M, p.a_row_bytes, MM))
     return cudaErrorInvalidValue;
-  if (a.quantized_out || a.f32_out)
+  if (a.quantized_out)
     m[6] = m[0];  // not used
-  else if (!make_out_map(&m[6], a.out, M, static_cast<uint64_t>(a.N)))
+  else if (!make_out_map(&m[6], a.out, M, static_cast<uint64_t>(a.N), a.f32_out != 0))
     return cudaErrorInvalidValue;
   const int sms = num_sms_for_current_device();
   const int64_t max_tiles = (cdiv64(a.M, MM) + a.G) * p.ct.tiles;

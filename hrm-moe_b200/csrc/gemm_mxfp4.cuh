@@ -264,6 +264,43 @@ __device__ __forceinline__ void store_bf16(const float (&v)[32], const Params& p
   }
 }
 
+// The same in fp32, as two boxes of 16 columns through the warp's one buffer.
+__device__ __forceinline__ void store_f32(const float (&v)[32], const Params& p,
+                                          const CUtensorMap* tmC, int col0, int64_t row,
+                                          int box_row, bool row_ok, bool box_full, uint32_t stg) {
+  const int lane = threadIdx.x & 31;
+  if (box_full) {
+    const uint32_t dst = stg + lane * 64;
+    const uint32_t sw = (lane >> 1) & 3;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (col0 + 16 * h >= p.N) break;
+      if (lane == 0) bulk_wait_group_read<0>();
+      __syncwarp();
+#pragma unroll
+      for (int c4 = 0; c4 < 4; ++c4) {
+        const float* f = v + 16 * h + 4 * c4;
+        st_shared_v4m(dst + ((c4 ^ sw) << 4),
+                      make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                                 __float_as_uint(f[3])));
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d(tmC, col0 + 16 * h, box_row, stg);
+        bulk_commit_group();
+      }
+    }
+  } else if (row_ok) {
+    float* orow = static_cast<float*>(p.out) + row * p.N + col0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col0 + 4 * i < p.N)  // N is a multiple of 8
+        *reinterpret_cast<float4*>(orow + 4 * i) =
+            make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  }
+}
+
 // A block of 32 values of one row -> its codes and scale.
 __device__ __forceinline__ uint4 quantize_block(const float (&v)[32], uint32_t& s) {
   float m = 0.0f;
@@ -325,7 +362,7 @@ __device__ __forceinline__ void load_chunk(uint32_t taddr, float (&v)[32]) {
 // What the epilogue writes (kF32: plain product only).
 enum Out { kBf16 = 0, kRecords = 1, kF32 = 2 };
 
-// Shared memory of the epilogue: a 2 KiB box per warp (bf16), or per row
+// Shared memory of the epilogue: a 2 KiB box per warp (bf16, fp32), or per row
 // quadrant two buffers of 32 rows x 48 bytes of codes and 4 of scales.
 constexpr int kQuadBuf = 32 * (16 * kMxTileChunks + 4);
 template <int OUT>
@@ -402,19 +439,12 @@ __device__ __forceinline__ void epilogue_tile(const Params& p, const CUtensorMap
       load_chunk<SWIGLU>(tquad + (SWIGLU ? 64 : 32) * c, v);
       if (c + kEpiWarps / 4 >= end) release();
       const int col0 = (chunk0 * kPer + c) * 32;
-      if constexpr (OUT == kF32) {
-        if (r < nrows) {
-          float* orow = static_cast<float*>(p.out) + (static_cast<int64_t>(row0) + r) * p.N + col0;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (col0 + 4 * i < p.N)  // N is a multiple of 8
-              *reinterpret_cast<float4*>(orow + 4 * i) =
-                  make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        }
-      } else {
-        store_bf16(v, p, tmC, col0, static_cast<int64_t>(row0) + r, row0 + quad * 32, r < nrows,
-                   (quad + 1) * 32 <= nrows, epi + w * kEpiBox);
-      }
+      const int64_t row = static_cast<int64_t>(row0) + r;
+      const bool full = (quad + 1) * 32 <= nrows;
+      if constexpr (OUT == kF32)
+        store_f32(v, p, tmC, col0, row, row0 + quad * 32, r < nrows, full, epi + w * kEpiBox);
+      else
+        store_bf16(v, p, tmC, col0, row, row0 + quad * 32, r < nrows, full, epi + w * kEpiBox);
     }
   }
 }
@@ -440,9 +470,10 @@ inline bool make_scale_map(CUtensorMap* map, const void* base, uint64_t atoms, u
   return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, atoms, 128, 512, box, 128,
                   CU_TENSOR_MAP_SWIZZLE_NONE);
 }
-inline bool make_out_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols) {
-  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, rows, cols, cols * 2, 32, 32,
-                  CU_TENSOR_MAP_SWIZZLE_64B);
+// Output [rows, cols], boxes of 32 rows x 64 bytes.
+inline bool make_out_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, bool f32) {
+  return make_map(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base,
+                  rows, cols, cols * (f32 ? 4 : 2), 32, f32 ? 16 : 32, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 inline Params make_params(const MxGemmArgs& a) {
   Params p;

@@ -600,12 +600,14 @@ cudaError_t launch_grouped_gemm_mxfp4_pair(const MxGemmArgs& a, cudaStream_t st)
     return cudaErrorInvalidValue;
   if (a.quantized_out)
     mc = ma;  // not used
-  else if (!make_out_map(&mc, a.out, static_cast<uint64_t>(a.M), static_cast<uint64_t>(a.N)))
+  else if (!make_out_map(&mc, a.out, static_cast<uint64_t>(a.M), static_cast<uint64_t>(a.N),
+                         a.f32_out != 0))
     return cudaErrorInvalidValue;
   const int sms = num_sms_for_current_device();
   const int64_t max_tiles = (cdiv64(a.M, 2 * MM) + a.G) * p.ct.tiles;
   int pairs = static_cast<int>(max_tiles < sms / 2 ? max_tiles : sms / 2);
   if (pairs < 1) pairs = 1;
+  if (a.f32_out) return launch_variant<false, kF32>(2 * pairs, ma, mb, mb1, ms, ms1, mr, mc, p, st);
   if (!a.swiglu) return launch_variant<false, kBf16>(2 * pairs, ma, mb, mb1, ms, ms1, mr, mc, p, st);
   if (a.quantized_out) return launch_variant<true, kRecords>(2 * pairs, ma, mb, mb1, ms, ms1, mr, mc, p, st);
   return launch_variant<true, kBf16>(2 * pairs, ma, mb, mb1, ms, ms1, mr, mc, p, st);

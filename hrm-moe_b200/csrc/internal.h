@@ -255,9 +255,9 @@ cudaError_t launch_mx_dequantize(const void* rows_in, int64_t rows, int K, int d
 cudaError_t launch_mx_pack_weight(const void* codes, int64_t code_stride, const void* scales,
                                   int64_t scale_stride, int G, int N, int K, int swiglu, void* out,
                                   cudaStream_t st);
-// out[t] = [final_in[t] +] sum_j w[t, j] * rows[pos[t, j]]; bf16 out, fp32
-// sums, rows in bf16 or (rows_f32) fp32.
-cudaError_t launch_combine_f32(const void* rows, int rows_f32, const int32_t* pos, const void* topk_w,
+// out[t] = [final_in[t] +] sum_j w[t, j] * rows[pos[t, j]]; fp32 rows and
+// sums, bf16 final_in and out.
+cudaError_t launch_combine_f32(const float* rows, const int32_t* pos, const void* topk_w,
                                int topk_w_is_f32, int64_t T, int d, int k, const void* final_in,
                                void* out, cudaStream_t st);
 struct MxGemmArgs {

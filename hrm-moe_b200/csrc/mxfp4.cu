@@ -192,13 +192,11 @@ pack_weight_kernel(const uint8_t* __restrict__ codes, int64_t code_stride,
 // y[t] = [final[t] +] sum over j of w[t, j] * row pos[t, j], in fp32, rounded
 // once.  Unlike combine_kernel, which repeats the roundings of the
 // reference's bf16 products and running sums, nothing here has a bf16
-// intermediate to repeat.  A warp per token, or per 32 chunks of 8 columns of
-// one; the k rows of a chunk are loaded before they are summed, in slot order.
-// F32: the rows are fp32.  Bound by reading the rows: XL 64x8 at T=16384
-// 453 MB in 82 us, 0.86 of the copy bandwidth.
-template <bool F32>
+// intermediate: the rows are the products' fp32 sums.  A warp per token, or
+// per 32 chunks of 8 columns of one; four rows of a chunk are loaded before
+// they are summed, in slot order.
 __global__ void __launch_bounds__(kQThreads, 4)
-combine_f32_kernel(const uint8_t* rows, const int32_t* pos, const void* topk_w, int topk_w_is_f32,
+combine_f32_kernel(const float* rows, const int32_t* pos, const void* topk_w, int topk_w_is_f32,
                    int64_t T, int row_chunks, int k, int warps_per_token, const uint4* final_in,
                    uint4* out) {
   grid_dependency_wait();
@@ -215,8 +213,7 @@ combine_f32_kernel(const uint8_t* rows, const int32_t* pos, const void* topk_w, 
     w = topk_w_is_f32 ? static_cast<const float*>(topk_w)[t * k + lane]
                       : bf16_bits_to_f32(static_cast<const uint16_t*>(topk_w)[t * k + lane]);
   }
-  constexpr int kBatch = F32 ? 4 : 8;
-  constexpr int kVecs = F32 ? 2 : 1;  // 16-byte loads of a chunk
+  constexpr int kBatch = 4;
   for (int c0 = cw * 32; c0 < row_chunks; c0 += warps_per_token * 32) {
     const int c = c0 + lane;
     const bool live = c < row_chunks;
@@ -230,7 +227,7 @@ combine_f32_kernel(const uint8_t* rows, const int32_t* pos, const void* topk_w, 
       for (int i = 0; i < 4; ++i) { acc[2 * i] = bf16_lo(q[i]); acc[2 * i + 1] = bf16_hi(q[i]); }
     }
     for (int j0 = 0; j0 < k; j0 += kBatch) {
-      uint4 v[kBatch][kVecs];
+      uint4 v[kBatch][2];
       float ws[kBatch];
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
@@ -239,25 +236,19 @@ combine_f32_kernel(const uint8_t* rows, const int32_t* pos, const void* topk_w, 
         const bool use = j0 + b < k && pj >= 0;
         if (!use) ws[b] = 0.0f;  // a dropped assignment adds nothing, whatever its weight
 #pragma unroll
-        for (int h = 0; h < kVecs; ++h)
+        for (int h = 0; h < 2; ++h)
           v[b][h] = live && use
-                        ? ld_16bytes(rows + ((static_cast<int64_t>(pj) * row_chunks + c) * kVecs + h) * 16)
+                        ? ld_16bytes(rows + (static_cast<int64_t>(pj) * row_chunks + c) * 8 + 4 * h)
                         : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
 #pragma unroll
-        for (int h = 0; h < kVecs; ++h) {
+        for (int h = 0; h < 2; ++h) {
           const uint32_t q[4] = {v[b][h].x, v[b][h].y, v[b][h].z, v[b][h].w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (F32) {
-              acc[4 * h + i] = fmaf(ws[b], __uint_as_float(q[i]), acc[4 * h + i]);
-            } else {
-              acc[2 * i] = fmaf(ws[b], bf16_lo(q[i]), acc[2 * i]);
-              acc[2 * i + 1] = fmaf(ws[b], bf16_hi(q[i]), acc[2 * i + 1]);
-            }
-          }
+          for (int i = 0; i < 4; ++i)
+            acc[4 * h + i] = fmaf(ws[b], __uint_as_float(q[i]), acc[4 * h + i]);
         }
       }
     }
@@ -316,18 +307,17 @@ cudaError_t launch_mx_pack_weight(const void* codes, int64_t code_stride, const 
   return cudaGetLastError();
 }
 
-cudaError_t launch_combine_f32(const void* rows, int rows_f32, const int32_t* pos,
-                               const void* topk_w, int topk_w_is_f32, int64_t T, int d, int k,
-                               const void* final_in, void* out, cudaStream_t st) {
+cudaError_t launch_combine_f32(const float* rows, const int32_t* pos, const void* topk_w,
+                               int topk_w_is_f32, int64_t T, int d, int k, const void* final_in,
+                               void* out, cudaStream_t st) {
   if (T == 0) return cudaSuccess;
   const int row_chunks = d / 8;
   // small T: a row over several warps, so that enough loads are in flight
   const int wpt = T < 4096 ? cdiv(row_chunks, 32) : 1;
   const int64_t blocks = cdiv64(T * wpt, kQThreads / 32);
-  return launch_pdl(kPdlCombine, rows_f32 ? combine_f32_kernel<true> : combine_f32_kernel<false>,
-                    dim3(static_cast<unsigned>(blocks)), dim3(kQThreads), 0, st,
-                    static_cast<const uint8_t*>(rows), pos, topk_w, topk_w_is_f32, T, row_chunks, k,
-                    wpt, static_cast<const uint4*>(final_in), static_cast<uint4*>(out));
+  return launch_pdl(kPdlCombine, combine_f32_kernel, dim3(static_cast<unsigned>(blocks)),
+                    dim3(kQThreads), 0, st, rows, pos, topk_w, topk_w_is_f32, T, row_chunks, k, wpt,
+                    static_cast<const uint4*>(final_in), static_cast<uint4*>(out));
 }
 
 }  // namespace hmoe

@@ -701,9 +701,9 @@ def experts_forward_mxfp4(hidden_states: torch.Tensor, selected_experts: torch.T
     """``experts_forward`` with MXFP4 expert weights; activations are quantised in the call.
 
     Returns a new [T, d] bf16 tensor, or adds into ``final_hidden_states`` in
-    place and returns it.  The products sum in fp32, an expert's output waits
-    in bf16 (in calls of up to 8 MiB of them: fp32), and a token's weighted sum
-    is fp32 rounded once.  Inference only.
+    place and returns it.  The products and a token's weighted sum of them are
+    fp32, rounded once, so a token's result does not depend on the other tokens
+    of the call.  Inference only.
     """
     if torch.is_grad_enabled() and (hidden_states.requires_grad or routing_weights.requires_grad or (
             final_hidden_states is not None and final_hidden_states.requires_grad)):

@@ -452,10 +452,9 @@ int hmoe_grouped_swiglu_mxfp4_dense(const void* x, int64_t x_stride, int32_t dty
  * N = hidden, K = intermediate).  bf16 hidden states, quantised within the
  * call; the routing is that of hmoe_ffn_forward.
  *   y[t] = bf16([final_in[t] +] sum_j w[t, j] * down(MXFP4(h)))
- * summed in fp32 and rounded once; the down products are rounded to bf16 in
- * between, except in small calls (tokens * top_k * hidden fp32 values of at
- * most 8 MiB), where they stay fp32.  final_in may be NULL (nothing added) or
- * y.
+ * with the down products and their sum in fp32, rounded once: a token's result
+ * does not depend on the other tokens of the call.  final_in may be NULL
+ * (nothing added) or y.
  */
 size_t hmoe_experts_mxfp4_workspace_bytes(const hmoe_shape* shape);
 int hmoe_experts_forward_mxfp4(const hmoe_shape* shape, const void* hidden,

@@ -13,7 +13,21 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a B200 (sm_100a) GPU")
 
 
+# Cases whose expected value is wrong, with the reason.  They stay as written and keep running;
+# strict: one that passes again is reported.
+WRONG_VALUES = {
+    "test_gpu_11_mxfp4.py::test_experts_forward[5000-256-96-16-4]":
+        "expects sum(w * bf16(e)) for calls over 8 MiB: each expert's output e rounded to bf16 before the "
+        "sum, which is up to 2^-8 sum(w |e|) from the value, with room for 2^-8 |sum| only; the sum is fp32 "
+        "(test_gpu_12_mxfp4_experts.py holds the same case to 64 bits)",
+}
+
+
 def pytest_collection_modifyitems(config, items):
+    for item in items:
+        for case, why in WRONG_VALUES.items():
+            if item.nodeid.endswith(case):
+                item.add_marker(pytest.mark.xfail(raises=AssertionError, strict=True, reason=why))
     try:
         import torch
         has_gpu = torch.cuda.is_available()
