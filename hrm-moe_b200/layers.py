@@ -24,6 +24,7 @@ quarter of the weight bytes).  Parameters and state dicts are untouched.
 """
 from __future__ import annotations
 
+import itertools
 import math
 from typing import Any, Literal, Optional, Sequence
 
@@ -84,6 +85,77 @@ def _valid_tokens(total_seqlen, tokens: int) -> int:
     return max(0, min(v, tokens))
 
 
+_DATA = torch.Tensor.data  # the attribute itself, which _PackedParameter overrides
+_EPOCHS = itertools.count()
+
+
+def _place(w: Tensor):
+    return w.untyped_storage()._cdata, w.storage_offset(), w.shape, w.stride(), w.dtype
+
+
+class _PackedParameter(nn.Parameter):
+    """A parameter of which a packed copy is in use.
+
+    In-place operations on a parameter count in its ``_version``; those through
+    its ``.data`` do not.  Here ``.data`` hands out views of one alias whose own
+    ``_version`` counts them, and other data in its place starts a new epoch.
+    A parameter becomes one (its ``__class__``) in :func:`_watch` and an
+    ``nn.Parameter`` again in :func:`_unwatch`, or when it is copied.
+    """
+
+    @property
+    def data(self):
+        return self._alias.detach()
+
+    @data.setter
+    def data(self, value):
+        before = _place(self)  # its storage lives in _alias until the new one is there
+        _DATA.__set__(self, value)
+        if _place(self) != before:
+            _start_epoch(self)
+
+    def _plain(self, data: Tensor) -> nn.Parameter:
+        p = nn.Parameter(data, self.requires_grad)
+        p.__dict__.update((k, v) for k, v in self.__dict__.items() if k not in ("_alias", "_epoch"))
+        return p
+
+    def __deepcopy__(self, memo):
+        if id(self) not in memo:
+            memo[id(self)] = nn.Parameter(self.detach().clone(memory_format=torch.preserve_format),
+                                          self.requires_grad)
+        return memo[id(self)]
+
+    def __reduce_ex__(self, proto):
+        return self._plain(self.detach()).__reduce_ex__(proto)
+
+
+def _start_epoch(w: _PackedParameter) -> None:
+    w._alias, w._epoch = _DATA.__get__(w), next(_EPOCHS)
+
+
+def _watch(w: nn.Parameter):
+    """Count the writes to ``w`` from now on; its state (None: they cannot be counted)."""
+    if w.is_inference() or type(w) not in (nn.Parameter, _PackedParameter):
+        return None
+    if type(w) is nn.Parameter:
+        w.__class__ = _PackedParameter
+        _start_epoch(w)
+    return _watched_state(w)
+
+
+def _unwatch(w: nn.Parameter) -> None:
+    if type(w) is _PackedParameter:
+        w.__class__ = nn.Parameter
+        del w._alias, w._epoch
+
+
+def _watched_state(w):
+    """Equal as long as nothing was written to ``w``; None: not watched (any more)."""
+    if type(w) is not _PackedParameter:
+        return None
+    return id(w), w._epoch, w._version, w._alias._version
+
+
 class SparseMoEGroupedExperts(nn.Module):
     """Experts backend with the reference's layout (models/layers.py:248-335)."""
 
@@ -108,30 +180,44 @@ class SparseMoEGroupedExperts(nn.Module):
         """Pack both weights as MXFP4 for inference (no counterpart in the reference).
 
         The packed copies belong to the weights as they are now: after the
-        weights change (an optimizer step, ``load_state_dict``, a move to
-        another device) inference raises until this is called again, or
-        :meth:`drop_quantized_experts` returns to the bf16 products.
+        weights change (an optimizer step, ``load_state_dict``, a write to the
+        parameter or through its ``.data``, a move to another device, another
+        parameter in its place) inference raises until this is called again, or
+        :meth:`drop_quantized_experts` returns to the bf16 products.  PyTorch
+        keeps no record of writes through a ``.data`` alias taken before this
+        call, or to the memory itself (another library, a replayed CUDA graph):
+        call this again after those.  Parameters made in inference mode, whose
+        writes it does not record at all, are refused.
         """
+        weights = self.gate_up_weight, self.down_weight
+        for w in weights:
+            if w.is_inference():
+                raise RuntimeError("quantize_experts() cannot see later writes to parameters that were "
+                                   "made in inference mode: make the module outside of it")
+            if type(w) not in (nn.Parameter, _PackedParameter):
+                raise TypeError(f"quantize_experts() takes plain parameters, got {type(w).__name__}")
         self._mxfp4 = (ops.pack_mxfp4_weight(self.gate_up_weight, swiglu=True),
                        ops.pack_mxfp4_weight(self.down_weight), self._weights_state(),
-                       (self.gate_up_weight, self.down_weight))  # kept: their ids stay theirs
+                       weights)  # kept: their ids stay theirs
 
     def drop_quantized_experts(self) -> None:
+        if self._mxfp4 is not None:
+            for w in self._mxfp4[3]:
+                _unwatch(w)
         self._mxfp4 = None
 
     def _weights_state(self):
-        # the parameter itself, its storage and its version: another parameter
-        # or .data in its place counts as a change too
-        return [(id(w), w.device, w.data_ptr(), None if w.is_inference() else w._version)
-                for w in (self.gate_up_weight, self.down_weight)]
+        """What :meth:`quantized` compares; from here on the parameters' ``.data`` is watched."""
+        return [_watch(w) for w in (self.gate_up_weight, self.down_weight)]
 
     def quantized(self):
         """The packed (gate_up, down) weights, or None.  Refuses stale ones."""
         if self._mxfp4 is None:
             return None
-        if self._mxfp4[2] != self._weights_state():
-            raise RuntimeError("the expert weights have changed since quantize_experts(): call it "
-                               "again, or drop_quantized_experts()")
+        for state, w in zip(self._mxfp4[2], (self.gate_up_weight, self.down_weight)):
+            if state is None or state != _watched_state(w):
+                raise RuntimeError("the expert weights have changed since quantize_experts(): call it "
+                                   "again, or drop_quantized_experts()")
         return self._mxfp4[:2]
 
     def forward(self, hidden_states: Tensor, selected_experts: Tensor, routing_weights: Tensor,
