@@ -174,7 +174,10 @@ class SparseMoEGroupedExperts(nn.Module):
             torch.empty((num_experts, 2 * intermediate_size, hidden_size), **kwargs), init_std_in))
         self.down_weight = nn.Parameter(trunc_normal_(
             torch.empty((num_experts, hidden_size, intermediate_size), **kwargs), init_std_out))
-        self._mxfp4 = None
+
+    # the packed weights while there are any; a class attribute, so that a module
+    # pickled before it existed has it too
+    _mxfp4 = None
 
     def quantize_experts(self) -> None:
         """Pack both weights as MXFP4 for inference (no counterpart in the reference).

@@ -164,3 +164,17 @@ def test_parameters_without_a_record_of_writes_are_refused(layers):
     m.experts.down_weight = Other(m.experts.down_weight.detach())
     with pytest.raises(TypeError, match="plain parameters"):
         m.quantize_experts()
+
+
+def test_a_module_pickled_without_packed_weights_loads(layers):
+    m = layers.SparseMoESwiGLU(32, 16, 4, 2, True, dtype=torch.bfloat16)
+    m.experts.__dict__.pop("_mxfp4", None)  # as pickled before the attribute existed
+    f = io.BytesIO()
+    torch.save(m, f)
+    f.seek(0)
+    old = torch.load(f, weights_only=False)
+    assert old.experts.quantized() is None
+    old.drop_quantized_experts()
+    assert _quantised(old.experts).quantized() == ("gate_up", "down")
+    old.drop_quantized_experts()
+    assert old.experts.quantized() is None and m.experts.quantized() is None
