@@ -141,6 +141,9 @@ grouped_gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
   const auto wait = [&](uint64_t& bar, uint32_t parity) {
     return mbar_wait_bounded(smem_u32(&bar), parity, abort, p.err, lim);
   };
+  const auto wait_warp = [&](uint64_t& bar, uint32_t parity) {
+    return mbar_wait_warp(smem_u32(&bar), parity, abort, p.err, lim);
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -277,7 +280,7 @@ grouped_gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
       uint4 v[4];
       for (int kb = 0; kb < nkb; ++kb) {
         if ((kb & 1) == 0) {
-          if (!wait(ctl.raw_full[raw.slot], raw.phase)) {
+          if (!wait_warp(ctl.raw_full[raw.slot], raw.phase)) {
             ok = false;
             break;
           }
@@ -285,7 +288,7 @@ grouped_gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
 #pragma unroll
           for (int h = 0; h < 4; ++h) v[h] = src[32 * h];
         }
-        if (!wait(ctl.empty[st.slot], st.phase ^ 1u)) {
+        if (!wait_warp(ctl.empty[st.slot], st.phase ^ 1u)) {
           ok = false;
           break;
         }
@@ -314,7 +317,7 @@ grouped_gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap tmA,
     int buf = 0;
     for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x) {
       const Tile t = decode_tile(ctl.tab, p, tile);
-      live = live && wait(ctl.acc_full[acc.slot], acc.phase);
+      live = live && wait_warp(ctl.acc_full[acc.slot], acc.phase);
       tc_fence_after();
       epilogue_tile<SWIGLU, OUT>(p, &tmC, w, tmem_base + acc.slot * kAccCols, t.row0,
                                   min(MM, t.row_end - t.row0), t.c0, t.nc, sbase + kOffEpi, buf, live,

@@ -116,6 +116,15 @@ __device__ __forceinline__ void st_shared_v4m(uint32_t addr, uint4 v) {
                : "memory");
 }
 
+// mbar_wait_bounded by a whole warp, with one answer for all its lanes: the
+// lanes read the barrier, the abort flag and the clock each for itself and may
+// differ near the limit, and a lane that left alone would leave the others at
+// the warp's next synchronisation without a bound.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort,
+                                               int* err, unsigned long long limit_ns) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort, err, limit_ns));
+}
+
 // A place in a ring of barriers, and the parity of its phase.
 struct Ring {
   int slot = 0;

@@ -503,12 +503,12 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
     };
     for (int i = 0; i < QR; ++i) fetch();
     for (; now.live; advance(now)) {
-      if (!mbar_wait_bounded(smem_u32(&ctl.raw_full[raw.slot]), raw.phase, abort, p.err, lim)) break;
+      if (!mbar_wait_warp(smem_u32(&ctl.raw_full[raw.slot]), raw.phase, abort, p.err, lim)) break;
       const uint4* src = reinterpret_cast<const uint4*>(smem + kOffRaw + raw.slot * 2048) + lane;
       uint4 v[4];
 #pragma unroll
       for (int h = 0; h < 4; ++h) v[h] = src[32 * h];
-      if (!mbar_wait_bounded(smem_u32(&ctl.sfa_empty[sa.slot]), sa.phase ^ 1u, abort, p.err, lim)) break;
+      if (!mbar_wait_warp(smem_u32(&ctl.sfa_empty[sa.slot]), sa.phase ^ 1u, abort, p.err, lim)) break;
       const uint32_t dst = sbase + kOffSfa + sa.slot * 2048 + lane * 16;
       st_shared_v4m(dst, make_uint4(v[0].x, v[1].x, v[2].x, v[3].x));
       st_shared_v4m(dst + kAtom, make_uint4(v[0].y, v[1].y, v[2].y, v[3].y));
@@ -526,9 +526,9 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
     // no copy into the landing ring is in flight when the CTA leaves (after an
     // early end), and no commit on its way to its barriers
     for (; raw.slot != in.slot || raw.phase != in.phase; raw.next(QR))
-      if (!mbar_wait_bounded(smem_u32(&ctl.raw_full[raw.slot]), raw.phase, &never, p.err, lim)) break;
+      if (!mbar_wait_warp(smem_u32(&ctl.raw_full[raw.slot]), raw.phase, &never, p.err, lim)) break;
     for (int i = 0; i < QR; ++i, sa.next(QR))
-      if (!mbar_wait_bounded(smem_u32(&ctl.sfa_empty[sa.slot]), sa.phase ^ 1u, &never, p.err, lim)) break;
+      if (!mbar_wait_warp(smem_u32(&ctl.sfa_empty[sa.slot]), sa.phase ^ 1u, &never, p.err, lim)) break;
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
     const int w = warp - 4;
@@ -541,7 +541,7 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
       const int my_row0 = un.row0 + static_cast<int>(rank) * MM;
       const int nrows = min(MM, un.row_end - my_row0);  // may be <= 0: nothing to store
       for (int t = un.t0; t < un.t1; ++t) {
-        live = live && mbar_wait_bounded(smem_u32(&ctl.acc_full[acc.slot]), acc.phase, abort, p.err, lim);
+        live = live && mbar_wait_warp(smem_u32(&ctl.acc_full[acc.slot]), acc.phase, abort, p.err, lim);
         tc_fence_after();
         epilogue_tile<SWIGLU, OUT>(
             p, &tmC, w, tmem_base + acc.slot * kAccCols, my_row0, nrows, p.ct.first(t), p.ct.count(t),
