@@ -116,10 +116,11 @@ SIGNATURES = {
                                           c_void_p]),
     "hmoe_grouped_linear_mxfp4_dense": (c_int, [c_void_p, c_int64, c_int32, c_void_p, c_void_p,
                                                 c_int64, c_int32, c_int32, c_int32, c_void_p,
-                                                c_void_p, c_void_p]),
+                                                c_void_p, c_void_p, c_size_t, c_void_p]),
     "hmoe_grouped_swiglu_mxfp4_dense": (c_int, [c_void_p, c_int64, c_int32, c_void_p, c_void_p,
                                                 c_int64, c_int32, c_int32, c_int32, c_int32,
-                                                c_void_p, c_void_p, c_void_p]),
+                                                c_void_p, c_void_p, c_void_p, c_size_t,
+                                                c_void_p]),
     "hmoe_experts_mxfp4_workspace_bytes": (c_size_t, [ShapeP]),
     "hmoe_experts_forward_mxfp4": (c_int, [ShapeP] + [c_void_p] * 10 + [c_size_t, c_void_p]),
     "hmoe_ffn_mxfp4_workspace_bytes": (c_size_t, [ShapeP]),

@@ -1368,28 +1368,60 @@ int mx_check_weight(int32_t groups, int32_t N, int32_t K, int swiglu) {
   return HMOE_OK;
 }
 
-int mx_grouped(const void* rows, const void* weight, const int32_t* tpe, int64_t M, int32_t N,
-               int32_t K, int32_t G, int swiglu, int quantized_out, void* output, void* workspace,
-               size_t workspace_bytes, void* stream) {
+// x [rows, K] that becomes records.
+struct MxDense {
+  const void* x;
+  int64_t stride;
+  int32_t dtype;
+  void* records;
+};
+
+int mx_check_dense(const MxDense& in) {
+  if (in.dtype != HMOE_DTYPE_BF16 && in.dtype != HMOE_DTYPE_F32)
+    return fail(HMOE_EINVAL, "unsupported dtype %d (bf16 = 0, f32 = 1)", in.dtype);
+  if (!in.x || !in.records) return fail(HMOE_EINVAL, "x and the memory for its records are required");
+  if (!aligned16(in.x) || !aligned16(in.records) ||
+      (in.stride * static_cast<int64_t>(elem_size(in.dtype))) % 16 != 0)
+    return fail(HMOE_EINVAL, "x, its rows and the records must be 16-byte aligned");
+  return HMOE_OK;
+}
+
+// A product on row records, or (dense) on an x that is quantised first, in
+// whose kernel the error word is cleared.  Everything is checked before the
+// first launch.
+int mx_grouped(const void* rows, const MxDense* dense, const void* weight, const int32_t* tpe, int64_t M,
+               int32_t N, int32_t K, int32_t G, int swiglu, int quantized_out, void* output,
+               void* workspace, size_t workspace_bytes, void* stream) {
   int rc = mx_check_weight(G, N, K, swiglu);
   if (rc) return rc;
   if (M < 0 || M > 0x7fffffffll) return fail(HMOE_EINVAL, "M must be in [0, 2^31), got %lld", (long long)M);
   if ((cdiv64(M, 128) + G) * cdiv64(mx_weight_rows(N, swiglu), 64) > 0x7fffffffll)
     return fail(HMOE_EINVAL, "too many output tiles");
-  if (M == 0) return HMOE_OK;
-  if (!rows || !weight || !tpe || !output) return fail(HMOE_EINVAL, "NULL tensor argument");
-  if (!aligned16(rows) || !aligned16(weight) || !aligned16(output))
-    return fail(HMOE_EINVAL, "rows, weight and output must be 16-byte aligned");
-  DeviceScope scope;
-  if ((rc = select_device(rows))) return rc;
-  int* err = nullptr;
-  if (workspace && workspace_bytes >= sizeof(int)) {
-    err = static_cast<int*>(workspace);
-    HMOE_CUDA(cudaMemsetAsync(err, 0, sizeof(int), static_cast<cudaStream_t>(stream)),
-              "reset error word");
+  if (reinterpret_cast<uintptr_t>(workspace) % sizeof(int) != 0)
+    return fail(HMOE_EINVAL, "workspace must be 4-byte aligned");
+  int* err = workspace && workspace_bytes >= sizeof(int) ? static_cast<int*>(workspace) : nullptr;
+  if (M > 0) {
+    if (dense) {
+      if ((rc = mx_check_dense(*dense))) return rc;
+      rows = dense->records;
+    }
+    if (!rows || !weight || !tpe || !output) return fail(HMOE_EINVAL, "NULL tensor argument");
+    if (!aligned16(rows) || !aligned16(weight) || !aligned16(output))
+      return fail(HMOE_EINVAL, "rows, weight and output must be 16-byte aligned");
+  } else if (!err) {
+    return HMOE_OK;
   }
+  DeviceScope scope;
+  if ((rc = select_device(M > 0 ? rows : err))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (err && (M == 0 || !dense))
+    HMOE_CUDA(cudaMemsetAsync(err, 0, sizeof(int), st), "reset error word");
+  if (M == 0) return HMOE_OK;
+  if (dense)
+    HMOE_CUDA(launch_mx_quantize(dense->x, M, K, dense->stride, dense->dtype, dense->records, err, st),
+              "quantize_mxfp4");
   MxGemmArgs a{rows, weight, tpe, output, M, N, K, G, swiglu, quantized_out, err};
-  const cudaError_t e = launch_grouped_gemm_mxfp4(a, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch_grouped_gemm_mxfp4(a, st);
   if (e != cudaSuccess) return cuda_fail(e, swiglu ? "grouped_swiglu_mxfp4" : "grouped_linear_mxfp4");
   return HMOE_OK;
 }
@@ -1475,12 +1507,11 @@ int hmoe_mxfp4_quantize(const void* x, int64_t rows, int32_t K, int64_t x_stride
   if (dtype != HMOE_DTYPE_BF16 && dtype != HMOE_DTYPE_F32)
     return fail(HMOE_EINVAL, "unsupported dtype %d (bf16 = 0, f32 = 1)", dtype);
   if (rows == 0) return HMOE_OK;
-  if (!x || !out) return fail(HMOE_EINVAL, "x and out are required");
-  if (!aligned16(x) || !aligned16(out) || (x_stride * static_cast<int64_t>(elem_size(dtype))) % 16 != 0)
-    return fail(HMOE_EINVAL, "x, its rows and out must be 16-byte aligned");
+  if ((rc = mx_check_dense(MxDense{x, x_stride, dtype, out}))) return rc;
   DeviceScope scope;
   if ((rc = select_device(x))) return rc;
-  HMOE_CUDA(launch_mx_quantize(x, rows, K, x_stride, dtype, out, static_cast<cudaStream_t>(stream)),
+  HMOE_CUDA(launch_mx_quantize(x, rows, K, x_stride, dtype, out, nullptr,
+                               static_cast<cudaStream_t>(stream)),
             "quantize_mxfp4");
   return HMOE_OK;
 }
@@ -1526,38 +1557,30 @@ int hmoe_mxfp4_pack_weight(const void* codes, int64_t code_stride, const void* s
   return HMOE_OK;
 }
 
-// The products on a dense x: quantised into `scratch` (M records) first.
-static int mx_grouped_dense(const void* x, int64_t x_stride, int32_t dtype, const void* weight,
-                            const int32_t* tpe, int64_t M, int32_t N, int32_t K, int32_t G,
-                            int swiglu, int quantized_out, void* output, void* scratch,
-                            void* stream) {
-  if (M > 0 && !scratch) return fail(HMOE_EINVAL, "scratch for the quantised rows is required");
-  const int rc = hmoe_mxfp4_quantize(x, M, K, x_stride, dtype, scratch, stream);
-  if (rc) return rc;
-  return mx_grouped(scratch, weight, tpe, M, N, K, G, swiglu, quantized_out, output, nullptr, 0, stream);
-}
-
 int hmoe_grouped_linear_mxfp4_dense(const void* x, int64_t x_stride, int32_t dtype,
                                     const void* weight, const int32_t* tokens_per_expert,
                                     int64_t M, int32_t N, int32_t K, int32_t groups, void* output,
-                                    void* scratch, void* stream) {
-  return mx_grouped_dense(x, x_stride, dtype, weight, tokens_per_expert, M, N, K, groups, 0, 0, output,
-                          scratch, stream);
+                                    void* scratch, void* workspace, size_t workspace_bytes,
+                                    void* stream) {
+  const MxDense in{x, x_stride, dtype, scratch};
+  return mx_grouped(nullptr, &in, weight, tokens_per_expert, M, N, K, groups, 0, 0, output, workspace,
+                    workspace_bytes, stream);
 }
 
 int hmoe_grouped_swiglu_mxfp4_dense(const void* x, int64_t x_stride, int32_t dtype,
                                     const void* w_gate_up, const int32_t* tokens_per_expert,
                                     int64_t M, int32_t I, int32_t K, int32_t groups,
                                     int32_t quantized_out, void* output, void* scratch,
-                                    void* stream) {
-  return mx_grouped_dense(x, x_stride, dtype, w_gate_up, tokens_per_expert, M, I, K, groups, 1,
-                          quantized_out ? 1 : 0, output, scratch, stream);
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+  const MxDense in{x, x_stride, dtype, scratch};
+  return mx_grouped(nullptr, &in, w_gate_up, tokens_per_expert, M, I, K, groups, 1,
+                    quantized_out ? 1 : 0, output, workspace, workspace_bytes, stream);
 }
 
 int hmoe_grouped_linear_mxfp4(const void* rows, const void* weight, const int32_t* tokens_per_expert,
                               int64_t M, int32_t N, int32_t K, int32_t groups, void* output,
                               void* workspace, size_t workspace_bytes, void* stream) {
-  return mx_grouped(rows, weight, tokens_per_expert, M, N, K, groups, 0, 0, output, workspace,
+  return mx_grouped(rows, nullptr, weight, tokens_per_expert, M, N, K, groups, 0, 0, output, workspace,
                     workspace_bytes, stream);
 }
 
@@ -1565,8 +1588,8 @@ int hmoe_grouped_swiglu_mxfp4(const void* rows, const void* w_gate_up,
                               const int32_t* tokens_per_expert, int64_t M, int32_t I, int32_t K,
                               int32_t groups, int32_t quantized_out, void* output, void* workspace,
                               size_t workspace_bytes, void* stream) {
-  return mx_grouped(rows, w_gate_up, tokens_per_expert, M, I, K, groups, 1, quantized_out ? 1 : 0,
-                    output, workspace, workspace_bytes, stream);
+  return mx_grouped(rows, nullptr, w_gate_up, tokens_per_expert, M, I, K, groups, 1,
+                    quantized_out ? 1 : 0, output, workspace, workspace_bytes, stream);
 }
 
 size_t hmoe_experts_mxfp4_workspace_bytes(const hmoe_shape* shape) {

@@ -245,9 +245,10 @@ cudaError_t launch_colsum_bf16(const void* m, int64_t T, int E, float* partial, 
                                void* out, cudaStream_t stream);
 
 // mxfp4.cu, gemm_mxfp4.cu (layouts: mxfp4.cuh) -----------------------------
-// x [rows, K] (row stride x_stride elements) -> row records.
+// x [rows, K] (row stride x_stride elements) -> row records.  clear_err (may
+// be NULL): this error word is cleared.
 cudaError_t launch_mx_quantize(const void* x, int64_t rows, int K, int64_t x_stride, int dtype,
-                               void* out, cudaStream_t st);
+                               void* out, int* clear_err, cudaStream_t st);
 // Row records -> values [rows, K].
 cudaError_t launch_mx_dequantize(const void* rows_in, int64_t rows, int K, int dtype, void* out,
                                  cudaStream_t st);

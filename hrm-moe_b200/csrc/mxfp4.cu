@@ -40,9 +40,11 @@ __device__ __forceinline__ int block_row(const RowSplit& sp, int i) {
 // else 16-byte loads, each of which may lie behind K (a multiple of 8).
 template <bool BF16, bool WIDE>
 __global__ void __launch_bounds__(kQThreads)
-quantize_kernel(const void* x, int64_t rows, int K, int64_t x_stride, RowSplit sp, uint8_t* out) {
+quantize_kernel(const void* x, int64_t rows, int K, int64_t x_stride, RowSplit sp, uint8_t* out,
+                int* clear_err) {
   grid_dependency_wait();  // launched early (launch_pdl)
   grid_launch_dependents();
+  if (clear_err && blockIdx.x == 0 && threadIdx.x == 0) *clear_err = 0;
   const int row_bytes = mx_row_bytes(K), cb = mx_code_bytes(K);
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * sp.rows_per_cta;
   const int nrows = static_cast<int>(rows - row0 < sp.rows_per_cta ? rows - row0 : sp.rows_per_cta);
@@ -267,7 +269,7 @@ unsigned stream_blocks(int64_t threads) {
 }  // namespace
 
 cudaError_t launch_mx_quantize(const void* x, int64_t rows, int K, int64_t x_stride, int dtype,
-                               void* out, cudaStream_t st) {
+                               void* out, int* clear_err, cudaStream_t st) {
   if (rows == 0) return cudaSuccess;
   const RowSplit sp = row_split(mx_num_scales(K));
   const int64_t ctas = cdiv64(rows, sp.rows_per_cta);
@@ -278,7 +280,7 @@ cudaError_t launch_mx_quantize(const void* x, int64_t rows, int K, int64_t x_str
   const auto kernel = bf16 ? (wide ? quantize_kernel<true, true> : quantize_kernel<true, false>)
                            : (wide ? quantize_kernel<false, true> : quantize_kernel<false, false>);
   return launch_pdl(kPdlDispatch, kernel, dim3(static_cast<unsigned>(ctas)), dim3(kQThreads), 0, st,
-                    x, rows, K, x_stride, sp, static_cast<uint8_t*>(out));
+                    x, rows, K, x_stride, sp, static_cast<uint8_t*>(out), clear_err);
 }
 
 cudaError_t launch_mx_dequantize(const void* rows_in, int64_t rows, int K, int dtype, void* out,

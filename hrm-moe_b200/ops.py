@@ -592,7 +592,7 @@ def pack_mxfp4_weight(weight, k: Optional[int] = None, swiglu: bool = False) -> 
 
 
 def _grouped_mxfp4(what: str, x, weight: Mxfp4Weight, tokens_per_expert: torch.Tensor, swiglu: bool,
-                   quantized: bool):
+                   quantized: bool, workspace: Optional[torch.Tensor]):
     if not isinstance(weight, Mxfp4Weight):
         raise TypeError(f"{what} takes a weight from pack_mxfp4_weight, got {type(weight).__name__}")
     if weight.swiglu != swiglu:
@@ -613,7 +613,13 @@ def _grouped_mxfp4(what: str, x, weight: Mxfp4Weight, tokens_per_expert: torch.T
     tpe = tokens_per_expert
     if tpe.numel() != G:
         raise ValueError(f"tokens_per_expert has {tpe.numel()} entries, weight has {G} groups")
-    dev = _require_cuda(rows, weight.data, tpe)
+    dev = _require_cuda(rows, weight.data, tpe, workspace)
+    ws, ws_bytes = None, 0
+    if workspace is not None:
+        if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < 4:
+            raise ValueError("workspace must be contiguous uint8 of at least 4 bytes, got "
+                             f"{workspace.dtype} {tuple(workspace.shape)}")
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel()
     M = rows.shape[0]
     if tpe.dtype != torch.int32 or not tpe.is_contiguous():
         tpe = tpe.to(torch.int32).contiguous()
@@ -628,40 +634,47 @@ def _grouped_mxfp4(what: str, x, weight: Mxfp4Weight, tokens_per_expert: torch.T
         args = (rows.data_ptr(), stride, code, weight.data.data_ptr(), tpe.data_ptr(), M, n, k, G)
         if swiglu:
             rc = lib.hmoe_grouped_swiglu_mxfp4_dense(*args, int(quantized), out.data_ptr(),
-                                                     scratch.data_ptr(), _raw_stream(dev))
-        else:
-            rc = lib.hmoe_grouped_linear_mxfp4_dense(*args, out.data_ptr(), scratch.data_ptr(),
+                                                     scratch.data_ptr(), ws, ws_bytes,
                                                      _raw_stream(dev))
+        else:
+            rc = lib.hmoe_grouped_linear_mxfp4_dense(*args, out.data_ptr(), scratch.data_ptr(), ws,
+                                                     ws_bytes, _raw_stream(dev))
     else:
         args = (rows.data_ptr(), weight.data.data_ptr(), tpe.data_ptr(), M, n, k, G)
         if swiglu:
-            rc = lib.hmoe_grouped_swiglu_mxfp4(*args, int(quantized), out.data_ptr(), None, 0,
+            rc = lib.hmoe_grouped_swiglu_mxfp4(*args, int(quantized), out.data_ptr(), ws, ws_bytes,
                                                _raw_stream(dev))
         else:
-            rc = lib.hmoe_grouped_linear_mxfp4(*args, out.data_ptr(), None, 0, _raw_stream(dev))
+            rc = lib.hmoe_grouped_linear_mxfp4(*args, out.data_ptr(), ws, ws_bytes, _raw_stream(dev))
     _lib.check(rc)
     return Mxfp4Rows._of(out, n) if quantized else out
 
 
-def grouped_linear_mxfp4(x, weight: Mxfp4Weight, tokens_per_expert: torch.Tensor) -> torch.Tensor:
+def grouped_linear_mxfp4(x, weight: Mxfp4Weight, tokens_per_expert: torch.Tensor,
+                         workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``grouped_linear`` on MXFP4 operands: [M, K] -> bf16 [M, N], sums in fp32.
 
     ``x`` is :class:`Mxfp4Rows` or a bf16 / fp32 tensor, which is quantised
     first; ``tokens_per_expert`` [G] counts each group's rows, contiguous in
     order.  Rows past the last group are not computed (their output is
-    uninitialised); groups past the last row are cut off.  Inference only.
+    uninitialised); groups past the last row are cut off.  ``workspace`` (uint8,
+    4 bytes or more): takes what the kernels report, a wait that gave up among
+    it, for :func:`workspace_status`.  Inference only.
     """
-    return _grouped_mxfp4("grouped_linear_mxfp4", x, weight, tokens_per_expert, False, False)
+    return _grouped_mxfp4("grouped_linear_mxfp4", x, weight, tokens_per_expert, False, False,
+                          workspace)
 
 
 def grouped_swiglu_mxfp4(x, weight: Mxfp4Weight, tokens_per_expert: torch.Tensor,
-                         quantized: bool = False):
+                         quantized: bool = False, workspace: Optional[torch.Tensor] = None):
     """``grouped_swiglu`` on MXFP4 operands: silu(gate) * up in fp32, [M, K] -> [M, I].
 
     Returns bf16, or with ``quantized`` the :class:`Mxfp4Rows` the down product
-    takes (quantised from the fp32 values).  Inference only.
+    takes (quantised from the fp32 values).  ``workspace`` as in
+    :func:`grouped_linear_mxfp4`.  Inference only.
     """
-    return _grouped_mxfp4("grouped_swiglu_mxfp4", x, weight, tokens_per_expert, True, quantized)
+    return _grouped_mxfp4("grouped_swiglu_mxfp4", x, weight, tokens_per_expert, True, quantized,
+                          workspace)
 
 
 @functools.lru_cache(maxsize=256)

@@ -420,7 +420,9 @@ int hmoe_mxfp4_pack_weight(const void* codes, int64_t code_stride, const void* s
  *   swiglu: h = silu(gate) * up in fp32; output [M, I] bf16, or with
  *           quantized_out [M] records of I (the next product's rows)
  * Rows past the last group are left as they were; groups past row M are cut
- * off.  N and K multiples of 8.  Workspace as hmoe_grouped_linear.
+ * off.  N and K multiples of 8.  workspace may be NULL; if not (4 bytes or
+ * more), its first word is cleared and then takes what the call's kernels
+ * report (hmoe_workspace_status).
  */
 int hmoe_grouped_linear_mxfp4(const void* rows, const void* weight,
                               const int32_t* tokens_per_expert, int64_t M, int32_t N, int32_t K,
@@ -439,12 +441,13 @@ int hmoe_grouped_swiglu_mxfp4(const void* rows, const void* w_gate_up,
 int hmoe_grouped_linear_mxfp4_dense(const void* x, int64_t x_stride, int32_t dtype,
                                     const void* weight, const int32_t* tokens_per_expert,
                                     int64_t M, int32_t N, int32_t K, int32_t groups, void* output,
-                                    void* scratch, void* stream);
+                                    void* scratch, void* workspace, size_t workspace_bytes,
+                                    void* stream);
 int hmoe_grouped_swiglu_mxfp4_dense(const void* x, int64_t x_stride, int32_t dtype,
                                     const void* w_gate_up, const int32_t* tokens_per_expert,
                                     int64_t M, int32_t I, int32_t K, int32_t groups,
                                     int32_t quantized_out, void* output, void* scratch,
-                                    void* stream);
+                                    void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * hmoe_experts_forward / hmoe_ffn_forward with packed MXFP4 expert weights

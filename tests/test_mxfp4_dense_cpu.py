@@ -1,0 +1,52 @@
+"""Refusals of the MXFP4 products on a dense input, and of their error word; no GPU needed."""
+import ctypes
+import errno
+import importlib
+
+import pytest
+import torch
+
+from _helpers import package
+
+
+@pytest.fixture(scope="module")
+def lib():
+    package()
+    return importlib.import_module("hrm-moe_b200._lib")
+
+
+def test_c_abi_refusals_of_the_dense_products(lib):
+    so = lib.load()
+    p = ctypes.c_void_p(4096)       # never followed: the call fails before it touches memory
+    odd = ctypes.c_void_p(4096 + 8)
+    lin, glu = so.hmoe_grouped_linear_mxfp4_dense, so.hmoe_grouped_swiglu_mxfp4_dense
+    #        x, stride, dtype, weight, counts, M, N, K, groups, [quantized,] output, scratch, ws, bytes, stream
+    cases = [
+        (lin, (p, 32, 0, p, p, 4, 12, 32, 2, p, p, None, 0, None), b"N must"),
+        (lin, (p, 32, 0, p, p, -1, 8, 32, 2, p, p, None, 0, None), b"M must"),
+        (lin, (p, 32, 2, p, p, 4, 8, 32, 2, p, p, None, 0, None), b"dtype"),
+        (lin, (None, 32, 0, p, p, 4, 8, 32, 2, p, p, None, 0, None), b"required"),
+        (lin, (p, 32, 0, p, p, 4, 8, 32, 2, p, None, None, 0, None), b"required"),
+        (lin, (p, 33, 0, p, p, 4, 8, 32, 2, p, p, None, 0, None), b"aligned"),
+        (lin, (p, 34, 1, p, p, 4, 8, 32, 2, p, p, None, 0, None), b"aligned"),
+        (lin, (odd, 32, 0, p, p, 4, 8, 32, 2, p, p, None, 0, None), b"aligned"),
+        (lin, (p, 32, 0, None, p, 4, 8, 32, 2, p, p, None, 0, None), b"NULL"),
+        (lin, (p, 32, 0, p, p, 4, 8, 32, 2, odd, p, None, 0, None), b"aligned"),
+        (lin, (p, 32, 0, p, p, 4, 8, 32, 2, p, p, ctypes.c_void_p(4098), 64, None), b"workspace"),
+        (glu, (p, 32, 0, p, None, 4, 8, 32, 2, 1, p, p, None, 0, None), b"NULL"),
+        (glu, (p, 32, 0, p, p, 4, 8, 32, 2, 0, p, p, ctypes.c_void_p(4098), 64, None), b"workspace"),
+        (so.hmoe_grouped_linear_mxfp4, (p, p, p, 4, 8, 32, 2, p, ctypes.c_void_p(4097), 64, None),
+         b"workspace"),
+    ]
+    for fn, args, word in cases:
+        assert fn(*args) == errno.EINVAL, (fn.__name__, args)
+        assert word in so.hmoe_last_error(), (fn.__name__, args, so.hmoe_last_error())
+    assert lin(None, 32, 0, None, None, 0, 8, 32, 2, None, None, None, 0, None) == 0
+
+
+def test_python_refuses_a_workspace_without_room_for_the_word(lib):
+    ops = importlib.import_module("hrm-moe_b200.ops")
+    w = ops.Mxfp4Weight(torch.zeros(16, dtype=torch.uint8), 2, 8, 64, False)
+    rows = ops.Mxfp4Rows(torch.zeros((4, 48), dtype=torch.uint8), 64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.grouped_linear_mxfp4(rows, w, torch.tensor([2, 2]), workspace=torch.zeros(64, dtype=torch.uint8))
