@@ -67,6 +67,15 @@ def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return torch.empty(max(int(nbytes), 1024), dtype=torch.uint8, device=device)
 
 
+def _check_router(w_router: torch.Tensor, router_bias: Optional[torch.Tensor], experts: int,
+                  hidden: int) -> None:
+    """The kernels take both sizes from the experts' weights: anything shorter would be read past its end."""
+    if tuple(w_router.shape) != (experts, hidden):
+        raise ValueError(f"router weight is {tuple(w_router.shape)}, expected {(experts, hidden)}")
+    if router_bias is not None and router_bias.numel() != experts:
+        raise ValueError(f"router bias has {router_bias.numel()} entries for {experts} experts")
+
+
 # ------------------------------------------------------------------ router --
 def router_topk(x: torch.Tensor, w_router: torch.Tensor, top_k: int, norm_topk_prob: bool,
                 router_bias: Optional[torch.Tensor] = None, return_logits: bool = False):
@@ -383,6 +392,7 @@ def ffn_forward(x: torch.Tensor, w_router: torch.Tensor, w_gate_up: torch.Tensor
     if tuple(w_gate_up.shape) != (E, 2 * I, d) or tuple(w_down.shape) != (E, d, I):
         raise ValueError(f"expert weights {tuple(w_gate_up.shape)} / {tuple(w_down.shape)} do not "
                          f"match hidden size {d} and {E} experts")
+    _check_router(w_router, router_bias, E, d)
     if out is None:
         out = (torch.zeros if accumulate else torch.empty)((T, d), dtype=dt, device=x.device)
     routing = None
@@ -774,8 +784,7 @@ def ffn_forward_mxfp4(x: torch.Tensor, w_router: torch.Tensor, w_gate_up: Mxfp4W
     dt = x.dtype
     shape, _, ws_bytes = _mxfp4_check(T, d, dt, top_k, w_gate_up, w_down, norm_topk_prob)
     E = w_gate_up.groups
-    if tuple(w_router.shape) != (E, d):
-        raise ValueError(f"router weight is {tuple(w_router.shape)}, expected {(E, d)}")
+    _check_router(w_router, router_bias, E, d)
     if out is None:
         out = (torch.zeros if accumulate else torch.empty)((T, d), dtype=dt, device=x.device)
     elif tuple(out.shape) != (T, d) or out.dtype != dt or not out.is_contiguous():
@@ -957,17 +966,16 @@ class CapturedFfn:
         self._mxfp4 = isinstance(w_gate_up, Mxfp4Weight) or isinstance(w_down, Mxfp4Weight)
         if self._mxfp4:
             self._shape, _, nbytes = _mxfp4_check(T, d, dt, top_k, w_gate_up, w_down, norm_topk_prob)
-            if tuple(w_router.shape) != (w_gate_up.groups, d):
-                raise ValueError(f"router weight is {tuple(w_router.shape)}, expected "
-                                 f"{(w_gate_up.groups, d)}")
+            _check_router(w_router, router_bias, w_gate_up.groups, d)
             w_gate_up, w_down = w_gate_up.data, w_down.data
             dev = _require_cuda(x, w_router, w_gate_up, w_down, router_bias)
         else:
-            dev = _require_cuda(x, w_router, w_gate_up, w_down, router_bias)
             I = w_gate_up.shape[1] // 2
             if tuple(w_gate_up.shape) != (E, 2 * I, d) or tuple(w_down.shape) != (E, d, I):
                 raise ValueError(f"expert weights {tuple(w_gate_up.shape)} / {tuple(w_down.shape)} "
                                  f"do not match hidden size {d} and {E} experts")
+            _check_router(w_router, router_bias, E, d)
+            dev = _require_cuda(x, w_router, w_gate_up, w_down, router_bias)
             self._shape = ctypes.byref(_lib.HmoeShape(T, d, E, I, top_k, dtype_code(dt),
                                                       1 if norm_topk_prob else 0))
             nbytes = _lib.load().hmoe_ffn_workspace_bytes(self._shape)

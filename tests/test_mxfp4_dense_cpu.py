@@ -50,3 +50,26 @@ def test_python_refuses_a_workspace_without_room_for_the_word(lib):
     rows = ops.Mxfp4Rows(torch.zeros((4, 48), dtype=torch.uint8), 64)
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.grouped_linear_mxfp4(rows, w, torch.tensor([2, 2]), workspace=torch.zeros(64, dtype=torch.uint8))
+
+
+def test_router_operands_of_other_sizes_are_refused(lib):
+    """A short bias or a narrow router weight would be read past its end: refused before any kernel."""
+    ops = importlib.import_module("hrm-moe_b200.ops")
+    E, d, I = 4, 64, 32
+    bf16 = dict(dtype=torch.bfloat16)
+    x, wr = torch.zeros((3, d), **bf16), torch.zeros((E, d), **bf16)
+    up = ops.Mxfp4Weight(torch.zeros(16, dtype=torch.uint8), E, I, d, True)
+    down = ops.Mxfp4Weight(torch.zeros(16, dtype=torch.uint8), E, d, I, False)
+    dense = torch.zeros((E, 2 * I, d), **bf16), torch.zeros((E, d, I), **bf16)
+    calls = [lambda r, b: ops.ffn_forward_mxfp4(x, r, up, down, 2, True, router_bias=b),
+             lambda r, b: ops.CapturedFfn(x, r, up, down, 2, True, b),
+             lambda r, b: ops.CapturedFfn(x, r, *dense, 2, True, b),
+             lambda r, b: ops.ffn_forward(x, r, *dense, 2, True, b)]
+    for f in calls:
+        for n in (1, E - 1, E + 1):
+            with pytest.raises(ValueError, match="router bias"):
+                f(wr, torch.zeros(n, **bf16))
+        with pytest.raises(ValueError, match="router weight"):
+            f(wr[:, :32], None)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            f(wr, torch.zeros(E, **bf16))
