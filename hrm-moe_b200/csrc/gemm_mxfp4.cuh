@@ -225,18 +225,22 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return r;
 }
 
-// silu(g) * u = g * u / (1 + 2^(-g log2 e)), in fp32 with the hardware's
-// approximate exponential and reciprocal (2^-22 relative each; the
-// denominator is at least 1, so flushing subnormals changes nothing).
+// silu(g) * u in fp32.  With a = 2^(-|g| log2 e) <= 1, the sigmoid of g is
+// 1 / (1 + a), or a / (1 + a) where g < 0: nothing overflows, and far on the
+// negative side it keeps a's subnormals (1 / (1 + 2^(|g| log2 e)) is zero from
+// g = -87.4 on, where silu(g) is still a normal number, times any u).
+// Approximate exponential and reciprocal, 2^-22 relative each.
 __device__ __forceinline__ float2 silu_mul2(float2 g, float2 u) {
-  const float2 x = mul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
-  float2 e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(x.x));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(x.y));
-  e = add2(e, make_float2(1.0f, 1.0f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
-  return mul2(mul2(g, r), u);
+  const float2 x = mul2(make_float2(fabsf(g.x), fabsf(g.y)),
+                        make_float2(-1.4426950408889634f, -1.4426950408889634f));
+  float2 a, r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(a.x) : "f"(x.x));
+  asm("ex2.approx.f32 %0, %1;" : "=f"(a.y) : "f"(x.y));
+  const float2 d = add2(a, make_float2(1.0f, 1.0f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));
+  const float2 n = make_float2(g.x < 0.0f ? g.x * a.x : g.x, g.y < 0.0f ? g.y * a.y : g.y);
+  return mul2(mul2(n, r), u);
 }
 
 // 32 output columns of one row, as a warp: rounded to bf16 and stored as a
