@@ -5,8 +5,8 @@
 //            MXFP4 records (the next product's input; h never exists in bf16)
 //
 // This file: one persistent CTA per SM, tiles of 128 rows x (up to) 192
-// columns, for groups of few rows.  (CTA pairs, for groups of many:
-// gemm_mxfp4_pair.cu.)  A k-block is 256 elements: a 128-byte swizzled row of
+// columns.  (CTA pairs, for much work in groups of many rows:
+// gemm_mxfp4_pair.cu; the rule is use_pairs.)  A k-block is 256 elements: a 128-byte swizzled row of
 // codes per operand row.  Warp 0 loads A (row records through a tensor map
 // whose row stride is the record; only the 32-row boxes that the group
 // reaches), A's scales as the records hold them, B and B's scale atoms; warp 2
@@ -392,14 +392,39 @@ bool make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint
 
 }  // namespace mx
 
+namespace {
+
+// Single CTAs or pairs: the same bits.  Pairs move fewer operand bytes, but
+// there are half as many of them, with tiles twice as high, and their first
+// tile takes longer.  So they win where each pair has several tiles to walk and
+// the groups fill them.  Products alone, equal groups, warm, us single / pair:
+//   gate_up, K=1536, 6 column tiles: 1 group of 2048 rows 8.0 / 10.8, 16384 22.2 / 21.8,
+//     65536 67.5 / 50.5; 8 groups, 8192 rows 14.2 / 17.4, 32768 38.5 / 31.7; 64 groups, 16384
+//     rows 28.1 / 28.3, 24576 35.7 / 34.4, 65536 73.8 / 56.4 (Zipf(1.2) groups 76.2 / 56.4)
+//   down, K=512, 8 tiles: 1 group of 8192 rows 10.4 / 12.0, 24576 23.0 / 21.1; 64 groups, 32768
+//     rows 31.9 / 32.1, 65536 53.8 / 51.5
+//   128 groups, down 448 -> 1280: 96 rows each 17.6 / 25.6, 160 25.7 / 26.0, 384 45.0 / 42.4
+//   K=2048, A no longer kept (when the pair kernel had that form): 8 groups, 8192 rows
+//     26.6 / 38.6, 98304 214 / 314
+// Seven 256-row tiles a pair and 160 rows a group part these; the worst miss was
+// the down product of 64 groups of 320 rows, 22.9 / 26.1 (a pair).
+bool use_pairs(const MxGemmArgs& a, int sms) {
+  if (mx_num_kblocks(a.K) > mx::kPairKBlocks) return false;
+  const int forced = forced_gemm_kernel();
+  if (forced >= 0) return forced == 1;
+  const int64_t tiles = mx_col_tiles(mx_weight_rows(a.N, a.swiglu)).tiles;
+  return a.M >= 160 * static_cast<int64_t>(a.G) && a.M * tiles >= 7ll * 256 * (sms / 2);
+}
+
+}  // namespace
+
 cudaError_t launch_grouped_gemm_mxfp4(const MxGemmArgs& a, cudaStream_t st) {
   using namespace mx;
   if (a.M == 0 || a.G == 0) return cudaSuccess;
   if (a.G > kMaxGroups || a.K % 8 != 0 || a.N % 8 != 0 || (a.f32_out && a.swiglu))
     return cudaErrorInvalidValue;
-  const int forced = forced_gemm_kernel();
-  if (forced >= 0 ? forced == 1 : a.M > 192 * static_cast<int64_t>(a.G))
-    return launch_grouped_gemm_mxfp4_pair(a, st);
+  const int sms = num_sms_for_current_device();
+  if (use_pairs(a, sms)) return launch_grouped_gemm_mxfp4_pair(a, st);
   Params p = make_params(a);
   const uint64_t cb = static_cast<uint64_t>(mx_code_bytes(a.K));
   const uint64_t M = static_cast<uint64_t>(a.M), wrows = static_cast<uint64_t>(a.G) * p.b_rows;
@@ -415,7 +440,6 @@ cudaError_t launch_grouped_gemm_mxfp4(const MxGemmArgs& a, cudaStream_t st) {
     m[6] = m[0];  // not used
   else if (!make_out_map(&m[6], a.out, M, static_cast<uint64_t>(a.N), a.f32_out != 0))
     return cudaErrorInvalidValue;
-  const int sms = num_sms_for_current_device();
   const int64_t max_tiles = (cdiv64(a.M, MM) + a.G) * p.ct.tiles;
   const unsigned grid = static_cast<unsigned>(max_tiles < sms ? max_tiles : sms);
   if (a.f32_out) return launch_variant<false, kF32>(grid, m, p, st);

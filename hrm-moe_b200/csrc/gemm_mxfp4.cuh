@@ -21,6 +21,7 @@ constexpr int kAccCols = 64 * kMxTileChunks;
 constexpr int kAccs = 2;
 constexpr int kEpiWarps = 12;  // three per lane quadrant
 constexpr int kThreads = 128 + 32 * kEpiWarps;
+constexpr int kPairKBlocks = 6;  // the most that the CTA-pair kernel takes
 constexpr int kSfaCols = 8;                  // TMEM columns of a k-block's scales
 constexpr int kSfbCols = 4 * kMxTileChunks;
 constexpr int kSfbBytes = kMxTileChunks * kAtom;
@@ -527,7 +528,7 @@ cudaError_t allow_smem(Kernel kernel, size_t bytes, int (&done)[64], std::mutex&
 
 }  // namespace mx
 
-// 256-row tiles on CTA pairs (gemm_mxfp4_pair.cu).
+// 256-row tiles on CTA pairs (gemm_mxfp4_pair.cu), K of at most kPairKBlocks.
 cudaError_t launch_grouped_gemm_mxfp4_pair(const MxGemmArgs& args, cudaStream_t st);
 
 }  // namespace hmoe

@@ -9,9 +9,9 @@
 // At the 4-bit rate (4 x bf16) operand traffic is what a plain tile loop is
 // bound by, so A stays: a pair takes a 256-row block and walks its column
 // tiles with the block's A in shared memory (a ring of six 256-element
-// k-blocks, K <= 1536; longer K reloads A per column tile through the same
-// ring), and a k-block's slot is refilled for the next row block as soon as
-// the last column tile has used it.  B streams through a ring of its own.
+// k-blocks: K <= 1536, longer K is the single-CTA kernel's), and a k-block's
+// slot is refilled for the next row block as soon as the last column tile has
+// used it.  B streams through a ring of its own.
 // XL gate_up at T=16384: 0.54 GB of operands to the SMs instead of 0.86 GB.
 //
 // TMEM (512 columns): two 192-column accumulators, six slots of A scales
@@ -37,7 +37,7 @@ namespace hmoe {
 namespace mx {
 namespace {
 
-constexpr int QA = 6;             // k-blocks of A
+constexpr int QA = kPairKBlocks;  // k-blocks of A
 constexpr int QB = 6;             // k-blocks of B
 constexpr int QR = 3;             // pairs of k-blocks of A's scales: as they come, and as atoms
 constexpr int kABytes = MM * kRowB;
@@ -270,7 +270,6 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
   const Walk share = share_of(ctl, p.ct.tiles, pair, npairs);
   const int kp = mx_padded_k(p.K);
   const int nkb = cdiv(kp, kMxKBlock);
-  const bool resident = nkb <= QA;
   volatile int* abort = &ctl.abort;
   int never = 0;
   const unsigned long long lim = p.wait_limit_ns;
@@ -291,7 +290,7 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
           const int brow = un.g * p.b_rows + c0 * 64 + static_cast<int>(rank) * nc * 32;
           const int srow = (un.g * p.b_chunks + c0) * nkb;
           const uint32_t bytes = 2 * nc * (kBChunkBytes + kAtom);  // both CTAs'
-          const bool load_a = t == un.t0 || !resident;
+          const bool load_a = t == un.t0;
           for (int kb = 0; kb < nkb; ++kb) {
             if (load_a) {
               if (!mbar_wait_bounded(smem_u32(&ctl.a_empty[a.slot]), a.phase ^ 1u, abort, p.err, lim)) {
@@ -345,11 +344,11 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
       Walk walk = share;
       Unit un{};
       while (ok && next_unit(ctl, G, p.ct.tiles, walk, un)) {
-        const int first = a.slot;  // the row block's first slot (resident)
+        const int first = a.slot;  // the row block's first slot
         for (int t = un.t0; ok && t < un.t1; ++t) {
           const int nc = p.ct.count(t);
-          const bool load_a = t == un.t0 || !resident;
-          const bool free_a = t == un.t1 - 1 || !resident;
+          const bool load_a = t == un.t0;
+          const bool free_a = t == un.t1 - 1;
           const uint32_t id0 = idesc_mxf4(2 * MM, 64 * nc, 0);
           if (!(ready & 2u) &&
               !mbar_wait_bounded(acc_empty + 8 * acc.slot, acc.phase ^ 1u, abort, p.err, lim)) {
@@ -416,7 +415,7 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
       while (ok && next_unit(ctl, G, p.ct.tiles, walk, un)) {
         for (int t = un.t0; ok && t < un.t1; ++t) {
           const int nc = p.ct.count(t);
-          const bool load_a = t == un.t0 || !resident;
+          const bool load_a = t == un.t0;
           for (int kb = 0; kb < nkb; ++kb) {
             if (load_a) {
               // a_full: the slot's TMEM columns are free as its codes are
@@ -465,22 +464,18 @@ grouped_gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmA,
     // pair when a unit's last tile ends.
     struct Step {  // two k-blocks of a unit's A
       Walk walk;
-      int rep, kb, row0, reps;
+      int kb, row0;
       bool live;
     };
     const auto start = [&](Step& st) {
       Unit un{};
       st.live = next_unit(ctl, G, p.ct.tiles, st.walk, un);
-      st.rep = st.kb = 0;
+      st.kb = 0;
       st.row0 = un.row0 + static_cast<int>(rank) * MM;
-      st.reps = resident ? 1 : un.t1 - un.t0;  // how often the unit's A is loaded
     };
     const auto advance = [&](Step& st) {
       st.kb += 2;
-      if (st.kb >= nkb) {
-        st.kb = 0;
-        if (++st.rep == st.reps) start(st);
-      }
+      if (st.kb >= nkb) start(st);
     };
     const int soff = mx_code_bytes(p.K);
     Ring in, raw, sa;
