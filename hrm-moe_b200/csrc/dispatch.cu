@@ -504,9 +504,9 @@ cudaError_t launch_dispatch_mxfp4(const int32_t* topk_idx, const void* x, int64_
   if (T == 0) return cudaSuccess;
   if (E > kMaxExperts) return cudaErrorInvalidValue;
   const bool wide = mx_wide(x, d);
-  // a row over several warps where the tokens alone are too few (as the copy)
+  // a row over several warps: a thread takes one block of it
   const bool small = dispatch_fits_one_block(T, k);
-  const int ncb = small || T < 4096 ? cdiv(mx_num_scales(d), 32) : 1;
+  const int ncb = cdiv(mx_num_scales(d), 32);
   const dim3 grid(static_cast<unsigned>(cdiv64(T * ncb, kPermThreads / 32)));
   uint4* out = static_cast<uint4*>(rows_sorted);
   if (small)
