@@ -536,6 +536,14 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Rows:
     return Mxfp4Rows._of(data, k)
 
 
+@functools.lru_cache(maxsize=256)
+def _mxfp4_weight_bytes(groups: int, n: int, k: int, swiglu: bool) -> int:
+    nbytes = _lib.load().hmoe_mxfp4_weight_bytes(groups, n, k, int(swiglu))
+    if nbytes == 0:
+        raise ValueError(_lib.last_error())
+    return nbytes
+
+
 class Mxfp4Weight:
     """An expert weight packed for the MXFP4 products (see :func:`pack_mxfp4_weight`).
 
@@ -547,6 +555,14 @@ class Mxfp4Weight:
 
     def __init__(self, data: torch.Tensor, groups: int, n: int, k: int, swiglu: bool):
         self.data, self.groups, self.n, self.k, self.swiglu = data, groups, n, k, swiglu
+
+    def _check(self) -> None:
+        """The kernels take the size of ``data`` from the other fields: any less would be read past its end."""
+        nbytes = _mxfp4_weight_bytes(self.groups, self.n, self.k, self.swiglu)
+        if self.data.dtype != torch.uint8 or self.data.numel() != nbytes or not self.data.is_contiguous():
+            raise ValueError(f"a packed weight [{self.groups}, {'2 x ' if self.swiglu else ''}{self.n}, "
+                             f"{self.k}] is {nbytes} contiguous bytes, got {self.data.dtype} "
+                             f"{tuple(self.data.shape)}")
 
     @property
     def device(self) -> torch.device:
@@ -591,9 +607,7 @@ def pack_mxfp4_weight(weight, k: Optional[int] = None, swiglu: bool = False) -> 
         raise ValueError("gate_up weight needs an even number of rows")
     n = N // 2 if swiglu else N
     lib = _lib.load()
-    nbytes = lib.hmoe_mxfp4_weight_bytes(G, n, int(k), int(swiglu))
-    if nbytes == 0:
-        raise ValueError(_lib.last_error())
+    nbytes = _mxfp4_weight_bytes(G, n, int(k), bool(swiglu))
     data = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _lib.check(lib.hmoe_mxfp4_pack_weight(_ptr(codes), codes.stride(1), _ptr(scales),
                                           scales.stride(1), G, n, int(k), int(swiglu), _ptr(data),
@@ -623,6 +637,7 @@ def _grouped_mxfp4(what: str, x, weight: Mxfp4Weight, tokens_per_expert: torch.T
     tpe = tokens_per_expert
     if tpe.numel() != G:
         raise ValueError(f"tokens_per_expert has {tpe.numel()} entries, weight has {G} groups")
+    weight._check()
     dev = _require_cuda(rows, weight.data, tpe, workspace)
     ws, ws_bytes = None, 0
     if workspace is not None:
@@ -712,6 +727,8 @@ def _mxfp4_check(T: int, d: int, dtype: torch.dtype, top_k: int, w_gate_up, w_do
         raise ValueError(
             f"expert weights [{E}, {'2 x ' if w_gate_up.swiglu else ''}{I}, {w_gate_up.k}] / "
             f"[{w_down.groups}, {w_down.n}, {w_down.k}] do not match hidden size {d}")
+    w_gate_up._check()
+    w_down._check()
     return _mxfp4_plan(T, d, E, I, top_k, bool(norm_topk_prob))
 
 

@@ -15,6 +15,11 @@ def lib():
     return importlib.import_module("hrm-moe_b200._lib")
 
 
+def _packed(ops, groups, n, k, swiglu):
+    return ops.Mxfp4Weight(torch.zeros(ops._lib.load().hmoe_mxfp4_weight_bytes(groups, n, k, int(swiglu)),
+                                       dtype=torch.uint8), groups, n, k, swiglu)
+
+
 def test_c_abi_refusals_of_the_dense_products(lib):
     so = lib.load()
     p = ctypes.c_void_p(4096)       # never followed: the call fails before it touches memory
@@ -46,7 +51,7 @@ def test_c_abi_refusals_of_the_dense_products(lib):
 
 def test_python_refuses_a_workspace_without_room_for_the_word(lib):
     ops = importlib.import_module("hrm-moe_b200.ops")
-    w = ops.Mxfp4Weight(torch.zeros(16, dtype=torch.uint8), 2, 8, 64, False)
+    w = _packed(ops, 2, 8, 64, False)
     rows = ops.Mxfp4Rows(torch.zeros((4, 48), dtype=torch.uint8), 64)
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.grouped_linear_mxfp4(rows, w, torch.tensor([2, 2]), workspace=torch.zeros(64, dtype=torch.uint8))
@@ -58,8 +63,7 @@ def test_router_operands_of_other_sizes_are_refused(lib):
     E, d, I = 4, 64, 32
     bf16 = dict(dtype=torch.bfloat16)
     x, wr = torch.zeros((3, d), **bf16), torch.zeros((E, d), **bf16)
-    up = ops.Mxfp4Weight(torch.zeros(16, dtype=torch.uint8), E, I, d, True)
-    down = ops.Mxfp4Weight(torch.zeros(16, dtype=torch.uint8), E, d, I, False)
+    up, down = _packed(ops, E, I, d, True), _packed(ops, E, d, I, False)
     dense = torch.zeros((E, 2 * I, d), **bf16), torch.zeros((E, d, I), **bf16)
     calls = [lambda r, b: ops.ffn_forward_mxfp4(x, r, up, down, 2, True, router_bias=b),
              lambda r, b: ops.CapturedFfn(x, r, up, down, 2, True, b),
@@ -73,3 +77,32 @@ def test_router_operands_of_other_sizes_are_refused(lib):
             f(wr[:, :32], None)
         with pytest.raises(RuntimeError, match="CUDA"):
             f(wr, torch.zeros(E, **bf16))
+
+
+def test_packed_weights_of_another_size_are_refused(lib):
+    """Fewer bytes than the fields say would be read past their end: refused before any kernel."""
+    ops = importlib.import_module("hrm-moe_b200.ops")
+    E, d, I = 4, 64, 32
+    bf16 = dict(dtype=torch.bfloat16)
+    x, wr, tpe = torch.zeros((3, d), **bf16), torch.zeros((E, d), **bf16), torch.tensor([3, 0, 0, 0])
+    sel, rw = torch.zeros((3, 2), dtype=torch.int32), torch.zeros((3, 2), **bf16)
+
+    def calls(up, down):
+        return [lambda: ops.grouped_swiglu_mxfp4(x, up, tpe), lambda: ops.grouped_linear_mxfp4(x[:, :I], down, tpe),
+                lambda: ops.experts_forward_mxfp4(x, sel, rw, up, down),
+                lambda: ops.ffn_forward_mxfp4(x, wr, up, down, 2, True),
+                lambda: ops.CapturedFfn(x, wr, up, down, 2, True)]
+
+    good = _packed(ops, E, I, d, True), _packed(ops, E, d, I, False)
+    for f in calls(*good):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            f()
+    cuts = [lambda t: t[:-16], lambda t: t[:16], lambda t: torch.cat((t, t)), lambda t: torch.cat((t, t))[::2],
+            lambda t: t.float()]
+    for cut in cuts:
+        bad = [ops.Mxfp4Weight(cut(w.data), w.groups, w.n, w.k, w.swiglu) for w in good]
+        for f in calls(*bad):
+            with pytest.raises(ValueError, match="packed weight"):
+                f()
+    with pytest.raises(ValueError, match="N must"):
+        ops.grouped_linear_mxfp4(x, ops.Mxfp4Weight(good[1].data, E, 12, d, False), tpe)
