@@ -187,3 +187,43 @@ def test_captured_products_take_new_inputs_and_counts():
             g.replay()
             assert torch.equal(out[:done], want[:done])
         ops.workspace_status(ws)
+
+
+# ------------------------------------------------------------------ modules --
+def _module(dtype):
+    L = importlib.import_module("hrm-moe_b200.layers")
+    torch.manual_seed(0)
+    return L.SparseMoESwiGLU(256, 96, 16, 4, True, device="cuda", dtype=dtype)
+
+
+@torch.no_grad()
+def test_a_module_serves_no_weights_that_were_written_over():
+    m = _module(torch.bfloat16)
+    x = _rand((40, 256), 1)
+    m.quantize_experts()
+    y = m(x)
+    for write in (lambda: m.experts.down_weight.data.mul_(2), lambda: m.experts.down_weight.data.copy_(
+            m.experts.down_weight.detach() * 0.5), lambda: m.experts.down_weight.mul_(2)):
+        write()
+        with pytest.raises(RuntimeError, match="changed"):
+            m(x)
+        m.quantize_experts()
+        m(x)
+    assert torch.equal(m(x).double(), 2 * y.double())  # a power of two moves every scale alike
+    m.drop_quantized_experts()
+    m.experts.down_weight.data.mul_(0.5)
+    m.quantize_experts()
+    assert torch.equal(m(x), y)
+
+
+@torch.no_grad()
+def test_fp32_parameters_serve_bf16_inputs():
+    ops = get_ops()
+    m = _module(torch.float32)
+    x = _rand((40, 256), 1)
+    m.quantize_experts()
+    want = ops.ffn_forward_mxfp4(x, m.gate.weight, ops.pack_mxfp4_weight(m.experts.gate_up_weight, swiglu=True),
+                                 ops.pack_mxfp4_weight(m.experts.down_weight), 4, True)
+    assert torch.equal(m(x), want)
+    with pytest.raises(TypeError, match="bf16"):
+        m(x.float())
