@@ -25,12 +25,13 @@
 // took 117 instead of 92 us.)
 //
 // Measured on XL 64x8 at T=16384 (131072 rows): gate_up with quantised output
-// 92 us for equal groups, 96 for ragged ones (4.5 PFLOP/s, tensor pipes 56 %
-// active), where four MMAs with fresh scales take 107 cycles of their nominal
-// 85 and the first loads, the change from one row block to the next and the
-// output stores leave the pipes idle the rest; down 94 us, bound by its
-// 403 MB of bf16 output (0.73 of the copy bandwidth with the operands' bytes).
-// The single-CTA kernel: 206 us for gate_up.
+// 92.6 us for equal groups (4.5 PFLOP/s, tensor pipes 56 % active), where an MMA
+// with fresh scales takes 107 cycles for its nominal 85 (average tile) and the
+// first loads, the change from one row block to the next and the output stores
+// leave the pipes idle the rest; down 93.6 us with bf16 output (466 MB, 0.77 of
+// the copy bandwidth) and 193 us with fp32 output (868 MB, 0.70), where neither
+// the tensor pipes (28 %) nor DRAM (54 %, 50 %) are full: the stores of the
+// epilogue do not drain faster.
 #include "gemm_mxfp4.cuh"
 
 namespace hmoe {

@@ -101,9 +101,9 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
   return r;
 }
 
-// Loads of what the kernel before may have written: volatile, and nothing in
-// these kernels is const __restrict__ or __ldg, so that the compiler moves no
-// load above griddepcontrol.wait.
+// Loads of what the kernel before may have written: volatile, so that the
+// compiler moves none of them above griddepcontrol.wait, whatever the
+// qualifiers of the pointer that a kernel passes in.
 __device__ __forceinline__ void ld_32bytes(const void* p, uint32_t* w) {
   asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]),

@@ -191,6 +191,8 @@ class SparseMoEGroupedExperts(nn.Module):
         call, or to the memory itself (another library, a replayed CUDA graph):
         call this again after those.  Parameters made in inference mode, whose
         writes it does not record at all, are refused.
+
+        Inputs are bf16 from then on, whatever the type of the parameters.
         """
         weights = self.gate_up_weight, self.down_weight
         for w in weights:
