@@ -1394,7 +1394,8 @@ int mx_grouped(const void* rows, const MxDense* dense, const void* weight, const
                void* workspace, size_t workspace_bytes, void* stream) {
   int rc = mx_check_weight(G, N, K, swiglu);
   if (rc) return rc;
-  if (M < 0 || M > 0x7fffffffll) return fail(HMOE_EINVAL, "M must be in [0, 2^31), got %lld", (long long)M);
+  if (M < 0 || M > 0x7fffffffll - 255)  // a 256-row block's end fits in int32
+    return fail(HMOE_EINVAL, "M must be in [0, 2^31 - 256], got %lld", (long long)M);
   if ((cdiv64(M, 128) + G) * cdiv64(mx_weight_rows(N, swiglu), 64) > 0x7fffffffll)
     return fail(HMOE_EINVAL, "too many output tiles");
   if (reinterpret_cast<uintptr_t>(workspace) % sizeof(int) != 0)

@@ -420,9 +420,9 @@ int hmoe_mxfp4_pack_weight(const void* codes, int64_t code_stride, const void* s
  *   swiglu: h = silu(gate) * up in fp32; output [M, I] bf16, or with
  *           quantized_out [M] records of I (the next product's rows)
  * Rows past the last group are left as they were; groups past row M are cut
- * off.  N and K multiples of 8.  workspace may be NULL; if not (4 bytes or
- * more), its first word is cleared and then takes what the call's kernels
- * report (hmoe_workspace_status).
+ * off.  N and K multiples of 8, M at most 2^31 - 256.  workspace may be
+ * NULL; if not (4 bytes or more), its first word is cleared and then takes what
+ * the call's kernels report (hmoe_workspace_status).
  */
 int hmoe_grouped_linear_mxfp4(const void* rows, const void* weight,
                               const int32_t* tokens_per_expert, int64_t M, int32_t N, int32_t K,

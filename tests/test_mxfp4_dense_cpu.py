@@ -106,3 +106,14 @@ def test_packed_weights_of_another_size_are_refused(lib):
                 f()
     with pytest.raises(ValueError, match="N must"):
         ops.grouped_linear_mxfp4(x, ops.Mxfp4Weight(good[1].data, E, 12, d, False), tpe)
+
+
+def test_row_counts_whose_blocks_pass_int32_are_refused(lib):
+    """The kernels count rows in 32 bits, up to the end of a row's block of 256."""
+    so = lib.load()
+    p = ctypes.c_void_p(4096)       # never followed
+    for M in (2 ** 31 - 255, 2 ** 31 - 1, 2 ** 31, 2 ** 40):
+        for fn, args in [(so.hmoe_grouped_linear_mxfp4, (p, p, p, M, 8, 8, 1, p, None, 0, None)),
+                         (so.hmoe_grouped_swiglu_mxfp4, (p, p, p, M, 8, 8, 1, 1, p, None, 0, None)),
+                         (so.hmoe_grouped_linear_mxfp4_dense, (p, 8, 0, p, p, M, 8, 8, 1, p, p, None, 0, None))]:
+            assert fn(*args) == errno.EINVAL and b"M must" in so.hmoe_last_error(), (fn.__name__, M)
