@@ -32,7 +32,8 @@ def _layer(T, d, I, E, k, seed):
 # T, d, I, E, k: outputs of a few KB to 50 MB, groups of few and of many rows,
 # more than 8 experts a token (the combine takes four at a time), up to the most there may be
 LARGE = [(1025, 512, 96, 16, 8), (5000, 256, 96, 16, 4), (8000, 64, 40, 4, 2), (700, 1000, 64, 24, 13),
-         (1500, 264, 72, 128, 32), (40, 96, 32, 128, 9)]
+         (1500, 264, 72, 128, 32), (40, 96, 32, 128, 9), (3000, 8, 8, 4, 2), (90000, 24, 8, 4, 1),
+         (129, 40, 16, 2, 1)]
 
 
 @pytest.mark.parametrize("T,d,I,E,k", LARGE)
